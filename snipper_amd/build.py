@@ -16,7 +16,10 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, os.path.basename(os.environ.get("SNIPPER_MSDA_LIB", "libsnipper_msda.so")))
 SOURCES = ["msda_capi.hip"]
 HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
-               "-Wall", "-Wno-cuda-compat", "-fno-gpu-rdc"] + os.environ.get("SNIPPER_HIPCC_EXTRA", "").split()
+               "-Wall", "-Wno-cuda-compat", "-fno-gpu-rdc",
+               # no packed float32 instructions (the compiler forms them from ordinary float code; some of their forms have given
+               # wrong results on this hardware).  The host pass does not know the feature and says so: harmless.
+               "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] + os.environ.get("SNIPPER_HIPCC_EXTRA", "").split()
 
 
 HASH_PATH = LIB_PATH + ".srchash"
