@@ -17,6 +17,18 @@ _FWD_ARGS = [c_void_p] * 6 + [c_int] * 7 + [c_void_p]          # stream, value, 
 _BWD_ARGS = [c_void_p] * 7 + [c_int] * 7 + [c_void_p] * 3      # stream, grad_out, value, ..., dims, 3 grads
 
 EXPORTS = {
+    # include/snipper_fp8.h
+    "snipper_fp8_quantize_workspace_bytes": ([c_int] * 3, c_size_t),
+    "snipper_fp8_quantize": ([c_void_p, c_void_p, c_int, c_longlong] + [c_int] * 4 + [c_void_p] * 4 + [c_int] + [c_void_p] * 6 +
+                             [c_size_t], c_int),
+    "snipper_fp8_matmul_workspace_bytes": ([c_int] * 4, c_size_t),
+    "snipper_fp8_matmul": ([c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int,
+                            c_void_p, c_int, c_void_p, c_size_t], c_int),
+    "snipper_layernorm_forward": ([c_void_p, c_void_p, c_int, c_longlong, c_void_p, c_void_p, c_int, c_int, c_int, ctypes.c_float] +
+                                  [c_void_p] * 5 + [c_int], c_int),
+    "snipper_layernorm_backward_workspace_bytes": ([c_int] * 2, c_size_t),
+    "snipper_layernorm_backward": ([c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int] +
+                                   [c_void_p] * 4 + [c_size_t], c_int),
     "snipper_msda_abi_version": ([], c_int),
     "snipper_msda_strerror": ([c_int], c_char_p),
     "snipper_msda_last_variant": ([], c_char_p),

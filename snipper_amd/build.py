@@ -14,7 +14,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 # (diagnostic builds: SNIPPER_MSDA_LIB = another file name in this directory, SNIPPER_HIPCC_EXTRA = extra compiler flags,
 #  e.g. -DWRES_STAMPS for the in-kernel cycle stamps of tools/wres_stamps.py; the product never sets them)
 LIB_PATH = os.path.join(PKG_DIR, os.path.basename(os.environ.get("SNIPPER_MSDA_LIB", "libsnipper_msda.so")))
-SOURCES = ["msda_capi.hip"]
+SOURCES = ["msda_capi.hip", "fp8_capi.hip"]
 HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
                "-Wall", "-Wno-cuda-compat", "-fno-gpu-rdc",
                # no packed float32 instructions (the compiler forms them from ordinary float code; some of their forms have given
@@ -70,10 +70,17 @@ def build_hip(force: bool = False, verbose: bool = False) -> str:
                     "available to rebuild it; set SNIPPER_ALLOW_STALE_LIB=1 to load it anyway")
             return LIB_PATH
         raise RuntimeError("hipcc not found: cannot build libsnipper_msda.so (gfx950)")
-    cmd = [hipcc] + HIPCC_FLAGS + ["-o", LIB_PATH + ".tmp"] + [os.path.join(CSRC, s) for s in SOURCES]
+    objects = [LIB_PATH + "." + s + ".o" for s in SOURCES]
+    cmds = [[hipcc] + [f for f in HIPCC_FLAGS if f != "-shared"] + ["-c", "-o", o, os.path.join(CSRC, s)] for o, s in zip(objects, SOURCES)]
+    link = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB_PATH + ".tmp"] + objects
     if verbose:
-        print(" ".join(cmd))
-    subprocess.check_call(cmd, cwd=CSRC)
+        print("\n".join(" ".join(c) for c in cmds + [link]))
+    running = [subprocess.Popen(c, cwd=CSRC) for c in cmds]           # the sources side by side
+    for p, c in [(p, c) for p, c in zip(running, cmds) if p.wait()]:
+        raise subprocess.CalledProcessError(p.returncode, c)
+    subprocess.check_call(link, cwd=CSRC)
+    for o in objects:
+        os.remove(o)
     os.replace(LIB_PATH + ".tmp", LIB_PATH)
     with open(HASH_PATH, "w") as fh:
         fh.write(source_hash() + "\n")

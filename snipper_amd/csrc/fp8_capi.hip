@@ -1,0 +1,236 @@
+// fp8_capi.hip -- extern "C" entry points of include/snipper_fp8.h: 8-bit block quantizers, the product of two such matrices, layer
+// norm of rows of any width.  As in msda_capi.hip: validate, pick a kernel, launch on the caller's stream, report errors; no
+// allocation, no synchronisation, no state.
+#include <hip/hip_runtime.h>
+#include <algorithm>
+#include <cstdint>
+#include <type_traits>
+
+#include "../../include/snipper_fp8.h"
+#include "gemm_fp8.cuh"
+#include "layernorm_rows.cuh"
+#include "quant_fp8.cuh"
+
+using namespace snipper::rows;
+
+namespace {
+
+constexpr int kMaxDim = 1 << 23;
+constexpr int kCUs = 256;
+constexpr int kLnMaxCols = 16384;
+
+int launch_status() {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? SNIPPER_OK : (int)e;
+}
+bool type_ok(int t) { return t == kF32 || t == kBF16 || t == kF16; }
+bool fmt_ok(int f) { return f == 0 || f == 1; }
+bool dim_ok(int n) { return n > 0 && n <= kMaxDim; }
+int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// f(T{}) for the element type of a code
+template <typename F>
+void with_type(int t, F &&f) {
+  if (t == kF32) f(float{});
+  else if (t == kBF16) f(bf16_t{});
+  else f(f16_t{});
+}
+template <typename F>
+void with_fmt(int fmt, F &&f) {
+  if (fmt == 0) f(std::integral_constant<int, 0>{});
+  else f(std::integral_constant<int, 1>{});
+}
+
+// ---- layer norm: lanes of a row and chunks of 8 elements of a lane
+template <typename F>
+void with_ln_shape(int cols, F &&f) {
+  using std::integral_constant;
+  if (cols <= 128) f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+  else if (cols <= 512) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+  else if (cols <= 1024) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+  else if (cols <= 2048) f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+  else if (cols <= 4096) f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+  else if (cols <= 8192) f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+  else f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+}
+int ln_rows_per_wg(int cols) { return cols <= 128 ? 16 : cols <= 2048 ? 4 : 1; }
+int ln_fwd_blocks(int rows, int cols) { return std::min(ceil_div(rows, ln_rows_per_wg(cols)), cols > 8192 ? 2 * kCUs : 8 * kCUs); }
+int ln_bwd_blocks(int rows, int cols) {
+  return std::min(ceil_div(rows, ln_rows_per_wg(cols)), cols > 8192 ? kCUs : cols > 2048 ? 2 * kCUs : 4 * kCUs);
+}
+
+// ---- product: which kernel, and how many pieces the K axis is cut into
+struct MmPlan {
+  int kind;                  // 0 few rows, 1 tiles of 128 x 128, 2 tiles of 256 x 256
+  int tiles, splits, per_split, waves, row_tiles;
+};
+MmPlan mm_plan(int M, int N, int K, bool exact) {
+  MmPlan p{};
+  const int steps = ceil_div(K, 128);
+  p.splits = 1;
+  p.per_split = steps;
+  if (M <= 64) {
+    p.row_tiles = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+    p.waves = std::max(1, std::min(16, steps / 4));
+    return p;
+  }
+  const long long big = (long long)ceil_div(M, 256) * ceil_div(N, 256);
+  p.kind = !exact && big >= kCUs ? 2 : 1;
+  const int edge = p.kind == 2 ? 256 : 128;
+  p.tiles = ceil_div(M, edge) * ceil_div(N, edge);
+  if (p.tiles < 2 * kCUs && steps >= 8) {
+    const int want = std::min(ceil_div(2 * kCUs, p.tiles), steps / 4);
+    p.per_split = ceil_div(ceil_div(steps, std::max(1, want)), 4) * 4;
+    p.splits = ceil_div(steps, p.per_split);
+  }
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t snipper_fp8_quantize_workspace_bytes(int rows, int cols, int with_colsum) {
+  if (!dim_ok(rows) || !dim_ok(cols) || !with_colsum) return 0;
+  return (size_t)ceil_div(rows, 128) * cols * sizeof(float);
+}
+
+int snipper_fp8_quantize(void *stream, const void *x, int x_dtype, long long ldx, int rows, int cols, int tile_rows, int fmt,
+                         const float *mean, const float *rstd, const void *gamma, const void *beta, int p_dtype, uint8_t *data,
+                         uint8_t *scale, uint8_t *data_t, uint8_t *scale_t, float *colsum, void *workspace, size_t workspace_bytes) {
+  if (!x || (!data && !data_t) || (data && !scale) || (data_t && !scale_t) || ((mean == nullptr) != (rstd == nullptr))) return SNIPPER_E_NULL;
+  if (!dim_ok(rows) || !dim_ok(cols) || ldx < cols || !type_ok(x_dtype) || !type_ok(p_dtype) || !fmt_ok(fmt)) return SNIPPER_E_SHAPE;
+  if (tile_rows != 1 && tile_rows != 128) return SNIPPER_E_SHAPE;
+  if (!mean && (gamma || beta)) return SNIPPER_E_SHAPE;
+  if (((uintptr_t)data | (uintptr_t)data_t) & 15 || ((uintptr_t)scale | (uintptr_t)scale_t) & 3) return SNIPPER_E_SHAPE;
+  if (colsum && (!workspace || workspace_bytes < snipper_fp8_quantize_workspace_bytes(rows, cols, 1))) return SNIPPER_E_SHAPE;
+  const QuantArgs a{x, ldx, rows, cols, mean, rstd, gamma, beta, p_dtype, data, scale, data_t, scale_t, colsum ? (float *)workspace : nullptr};
+  hipStream_t st = (hipStream_t)stream;
+  if (tile_rows == 1 && !data_t && !mean && !colsum) {
+    const long long wgs = ((long long)rows * ceil_div(cols, 512) + 3) / 4;
+    const dim3 grid((unsigned)std::min<long long>(wgs, 16 * kCUs));
+    with_type(x_dtype, [&](auto t) {
+      with_fmt(fmt, [&](auto f) { hipLaunchKernelGGL((quant_rows_kernel<decltype(t), decltype(f)::value>), grid, dim3(256), 0, st, a); });
+    });
+    return launch_status();
+  }
+  const int rb = ceil_div(rows, 128);
+  const dim3 grid(ceil_div(cols, 128), std::min(rb, 32768), ceil_div(rb, 32768));
+  with_type(x_dtype, [&](auto t) {
+    with_fmt(fmt, [&](auto f) {
+      using T = decltype(t);
+      constexpr int F = decltype(f)::value;
+      if (tile_rows == 128) {
+        if (mean) hipLaunchKernelGGL((quant_tile_kernel<T, F, true, true>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((quant_tile_kernel<T, F, true, false>), grid, dim3(256), 0, st, a);
+      } else {
+        if (mean) hipLaunchKernelGGL((quant_tile_kernel<T, F, false, true>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((quant_tile_kernel<T, F, false, false>), grid, dim3(256), 0, st, a);
+      }
+    });
+  });
+  if (colsum) hipLaunchKernelGGL(colsum_parts_kernel, dim3(ceil_div(cols, 8)), dim3(256), 0, st, (const float *)workspace, rb, cols, colsum);
+  return launch_status();
+}
+
+size_t snipper_fp8_matmul_workspace_bytes(int M, int N, int K, int out_dtype) {
+  if (!dim_ok(M) || !dim_ok(N) || !dim_ok(K) || !type_ok(out_dtype)) return 0;
+  const MmPlan p = mm_plan(M, N, K, out_dtype == kF32);
+  return p.splits > 1 ? (size_t)p.splits * M * N * sizeof(float) : 0;
+}
+
+int snipper_fp8_matmul(void *stream, const uint8_t *A, const uint8_t *a_scale, int a_fmt, const uint8_t *B, const uint8_t *b_scale,
+                       int b_fmt, int M, int N, int K, const void *bias, int bias_dtype, int relu, void *out, int out_dtype,
+                       void *workspace, size_t workspace_bytes) {
+  if (!A || !a_scale || !B || !b_scale || !out) return SNIPPER_E_NULL;
+  if (!dim_ok(M) || !dim_ok(N) || !dim_ok(K) || !fmt_ok(a_fmt) || !fmt_ok(b_fmt) || !type_ok(out_dtype) || !type_ok(bias_dtype)) return SNIPPER_E_SHAPE;
+  if (((uintptr_t)A | (uintptr_t)B) & 15 || ((uintptr_t)a_scale | (uintptr_t)b_scale) & 3) return SNIPPER_E_SHAPE;
+  const bool exact = out_dtype == kF32;
+  const MmPlan p = mm_plan(M, N, K, exact);
+  const size_t need = snipper_fp8_matmul_workspace_bytes(M, N, K, out_dtype);
+  if (need && (!workspace || workspace_bytes < need)) return SNIPPER_E_SHAPE;
+  const MmArgs a{A, a_scale, B, b_scale, M, N, ceil_div(K, 128), bias, bias_dtype, relu, out, out_dtype,
+                 p.splits > 1 ? (float *)workspace : nullptr, p.splits, p.per_split};
+  hipStream_t st = (hipStream_t)stream;
+  with_fmt(a_fmt, [&](auto fa) {
+    with_fmt(b_fmt, [&](auto fb) {
+      constexpr int FA = decltype(fa)::value, FB = decltype(fb)::value;
+      auto go = [&](auto ex) {
+        constexpr bool E = decltype(ex)::value;
+        if (p.kind == 0) {
+          const dim3 grid(ceil_div(N, 16), ceil_div(M, 16 * p.row_tiles)), block(64 * p.waves);
+          const size_t lds = (size_t)p.waves * p.row_tiles * 64 * 16;
+          if (p.row_tiles == 1) hipLaunchKernelGGL((mm_rows_kernel<FA, FB, E, 1>), grid, block, lds, st, a);
+          else if (p.row_tiles == 2) hipLaunchKernelGGL((mm_rows_kernel<FA, FB, E, 2>), grid, block, lds, st, a);
+          else hipLaunchKernelGGL((mm_rows_kernel<FA, FB, E, 4>), grid, block, lds, st, a);
+        } else if (p.kind == 1) {
+          hipLaunchKernelGGL((mm_tile_kernel<FA, FB, E, 2, 2, 4, 4>), dim3(p.tiles, p.splits), dim3(256), 0, st, a);
+        } else if constexpr (!E) {
+          hipLaunchKernelGGL((mm_tile_kernel<FA, FB, false, 2, 4, 8, 4>), dim3(p.tiles, p.splits), dim3(512), 0, st, a);
+        }
+      };
+      if (exact) go(std::true_type{});
+      else go(std::false_type{});
+    });
+  });
+  if (p.splits > 1) {
+    const long long units = (long long)M * ((N + 3) / 4);
+    hipLaunchKernelGGL(mm_join_kernel, dim3((unsigned)std::min<long long>((units + 255) / 256, 16 * kCUs)), dim3(256), 0, st, a);
+  }
+  return launch_status();
+}
+
+int snipper_layernorm_forward(void *stream, const void *x, int x_dtype, long long ldx, const void *gamma, const void *beta, int p_dtype,
+                              int rows, int cols, float eps, void *y, float *mean, float *rstd, uint8_t *data, uint8_t *scale, int fmt) {
+  if (!x || (!y && !mean && !data) || ((mean == nullptr) != (rstd == nullptr)) || ((data == nullptr) != (scale == nullptr))) return SNIPPER_E_NULL;
+  if (rows <= 0 || cols <= 0 || cols > kLnMaxCols || ldx < cols || !type_ok(x_dtype) || !type_ok(p_dtype) || !fmt_ok(fmt) || !(eps >= 0.f))
+    return SNIPPER_E_SHAPE;
+  if ((uintptr_t)data & 15 || (uintptr_t)scale & 3) return SNIPPER_E_SHAPE;
+  LnRowsArgs a{};
+  a.x = x; a.ldx = ldx; a.gamma = gamma; a.beta = beta; a.p_dtype = p_dtype; a.R = rows; a.C = cols; a.eps = eps;
+  a.y = y; a.mean = mean; a.rstd = rstd; a.data = data; a.scale = scale;
+  const dim3 grid(ln_fwd_blocks(rows, cols));
+  hipStream_t st = (hipStream_t)stream;
+  with_type(x_dtype, [&](auto t) {
+    with_ln_shape(cols, [&](auto lpr, auto nit) {
+      using T = decltype(t);
+      constexpr int L = decltype(lpr)::value, I = decltype(nit)::value;
+      if (!data) hipLaunchKernelGGL((ln_rows_fwd_kernel<T, L, I, -1>), grid, dim3(ln_threads(L)), 0, st, a);
+      else if (fmt == 0) hipLaunchKernelGGL((ln_rows_fwd_kernel<T, L, I, 0>), grid, dim3(ln_threads(L)), 0, st, a);
+      else hipLaunchKernelGGL((ln_rows_fwd_kernel<T, L, I, 1>), grid, dim3(ln_threads(L)), 0, st, a);
+    });
+  });
+  return launch_status();
+}
+
+size_t snipper_layernorm_backward_workspace_bytes(int rows, int cols) {
+  if (rows <= 0 || cols <= 0 || cols > kLnMaxCols) return 0;
+  return (size_t)ln_bwd_blocks(rows, cols) * 2 * cols * sizeof(float);
+}
+
+int snipper_layernorm_backward(void *stream, const void *g, const void *x, int x_dtype, long long ldx, const float *mean, const float *rstd,
+                               const void *gamma, int p_dtype, int rows, int cols, void *dx, void *dgamma, void *dbeta, void *workspace,
+                               size_t workspace_bytes) {
+  if (((dgamma == nullptr) != (dbeta == nullptr)) || (!dx && !dgamma)) return SNIPPER_E_NULL;
+  if (rows < 0 || cols <= 0 || cols > kLnMaxCols || ldx < cols || !type_ok(x_dtype) || !type_ok(p_dtype)) return SNIPPER_E_SHAPE;
+  if (rows > 0 && (!g || !x || !mean || !rstd)) return SNIPPER_E_NULL;
+  if (rows > 0 && dgamma && (!workspace || workspace_bytes < snipper_layernorm_backward_workspace_bytes(rows, cols))) return SNIPPER_E_SHAPE;
+  const int blocks = rows > 0 ? ln_bwd_blocks(rows, cols) : 0;
+  LnRowsArgs a{};
+  a.x = x; a.ldx = ldx; a.gamma = gamma; a.p_dtype = p_dtype; a.R = rows; a.C = cols;
+  a.mean = const_cast<float *>(mean); a.rstd = const_cast<float *>(rstd);
+  a.g = g; a.dx = dx; a.part = dgamma ? (float *)workspace : nullptr;
+  hipStream_t st = (hipStream_t)stream;
+  if (rows > 0)
+    with_type(x_dtype, [&](auto t) {
+      with_ln_shape(cols, [&](auto lpr, auto nit) {
+        constexpr int L = decltype(lpr)::value, I = decltype(nit)::value;
+        hipLaunchKernelGGL((ln_rows_bwd_kernel<decltype(t), L, I>), dim3(blocks), dim3(ln_threads(L)), 0, st, a);
+      });
+    });
+  if (dgamma)
+    hipLaunchKernelGGL(ln_rows_join_kernel, dim3(ceil_div(2 * cols, 8)), dim3(256), 0, st, (const float *)workspace, blocks, cols, dgamma, dbeta, p_dtype);
+  return launch_status();
+}
+
+}  // extern "C"

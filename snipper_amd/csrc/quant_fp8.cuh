@@ -1,0 +1,217 @@
+// quant_fp8.cuh -- matrices into 8-bit blocks with a power-of-two scale for each 128 elements (gfx950); format: include/snipper_fp8.h.
+//
+//   q = round(x / 2^e),   e = smallest exponent with max|x| / 2^e <= largest value of the type,   over 128 elements of a row, of a
+//   column, or of a 128 x 128 tile.
+//
+// Powers of two make the division exact, so a result is the input rounded once, and they are what the block-scaled matrix
+// instructions of gemm_fp8.cuh take as they are.  The scale's exponent comes from the bits of the maximum, not from a logarithm.
+// Bound by HBM: one read of x, one byte written per element and form.
+#pragma once
+#include "rows_common.cuh"
+
+namespace snipper {
+namespace rows {
+
+struct QuantArgs {
+  const void *x; long long ldx;
+  int R, C;                                  // rows, columns
+  const float *mean, *rstd;                  // [R] or null: normalise first
+  const void *gamma, *beta; int p_dtype;     // [C] or null
+  uint8_t *data, *scale;                     // [R][P], [R][Q] or null
+  uint8_t *data_t, *scale_t;                 // [C][Pt], [C][Qt] or null
+  float *part;                               // [ceil(R / 128)][C] or null: sums over the rows of a tile
+};
+
+__host__ __device__ __forceinline__ long long pitch_of(int cols) { return (long long)((cols + 127) / 128) * 128; }
+__host__ __device__ __forceinline__ long long scales_of(int cols) { return (long long)((cols + 511) / 512) * 4; }
+
+// ---- rows only.  A wave takes 512 consecutive elements of a row, 8 per lane: four blocks, so that it writes a whole 32-bit word of
+// scales; 16 lanes share a block.
+template <typename T, int FMT>
+__global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int groups = (a.C + 511) >> 9;
+  const long long units = (long long)a.R * groups;
+  const long long P = pitch_of(a.C), Q = scales_of(a.C);
+  for (long long u = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); u < units; u += (long long)gridDim.x * 4) {
+    const long long row = u / groups;
+    const int g = (int)(u - row * groups), c = g * 512 + lane * 8;
+    float v[8];
+    load8((const T *)a.x + row * a.ldx + c, a.C - c, v);
+    unsigned m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, mag(v[j]));
+    const int byte = scale_byte<FMT>(max16(m));
+    const float f = inv_scale(byte);
+    if (c < P) {
+      const u32x2 w = {pack4<FMT>(v[0] * f, v[1] * f, v[2] * f, v[3] * f), pack4<FMT>(v[4] * f, v[5] * f, v[6] * f, v[7] * f)};
+      *(u32x2 *)(a.data + row * P + c) = w;
+    }
+    const unsigned b0 = __shfl(byte, 0, 64), b1 = __shfl(byte, 16, 64), b2 = __shfl(byte, 32, 64), b3 = __shfl(byte, 48, 64);
+    if (lane == 0) *(unsigned *)(a.scale + row * Q + g * 4) = b0 | (b1 << 8) | (b2 << 16) | (b3 << 24);
+  }
+}
+
+// ---- both forms from one read.  A workgroup of four waves holds a 128 x 128 tile in registers: lane (i, l) = (lane >> 4, lane & 15)
+// of wave w the columns 8 l .. 8 l + 7 of rows 32 w + 16 h + 4 i + k (h < 2, k < 4).  Four consecutive rows in one lane make a 32-bit
+// word of the transposed form, which crosses LDS once (16-byte pieces XORed by the column's octet: reads are free of bank conflicts,
+// writes two-way) and is written as whole 128-byte lines.
+template <typename T, int FMT, bool TILE, bool NORM>
+__global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs a) {
+  __shared__ __attribute__((aligned(16))) unsigned img[128 * 32];
+  __shared__ unsigned cmax[4][128];
+  __shared__ float csum[4][128];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, i4 = lane >> 4;
+  const int c0 = blockIdx.x * 128, c = c0 + 8 * l;
+  const int rb = blockIdx.y + (int)blockIdx.z * 32768;
+  const long long r0 = (long long)rb * 128;
+  if (r0 >= a.R) return;                                   // (the whole workgroup)
+  float v[2][4][8];
+  float gm[8], bt[8];
+  if constexpr (NORM) {
+    load_param8(a.gamma, a.p_dtype, c, a.C - c, 1.f, gm);
+    load_param8(a.beta, a.p_dtype, c, a.C - c, 0.f, bt);
+  }
+  const int n = a.C - c;                                     // columns this lane has (8 of them unless the matrix ends)
+  const long long rl = r0 + 32 * wave + 4 * i4;
+  auto row_of = [&](int h, int k) { return rl + 16 * h + k; };
+  if (n >= 8) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const long long r = row_of(h, k) < a.R ? row_of(h, k) : a.R - 1;
+        load8((const T *)a.x + r * a.ldx + c, 8, v[h][k]);
+      }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const long long r = row_of(h, k) < a.R ? row_of(h, k) : a.R - 1;
+          v[h][k][j] = j < n ? (float)((const T *)a.x)[r * a.ldx + c + j] : 0.f;
+        }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool in = row_of(h, k) < a.R;
+      if constexpr (NORM) {
+        const float mu = in ? a.mean[row_of(h, k)] : 0.f, rs = in ? a.rstd[row_of(h, k)] : 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[h][k][j] = j < n ? (v[h][k][j] - mu) * rs * gm[j] + bt[j] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[h][k][j] = in ? v[h][k][j] : 0.f;
+    }
+  const long long P = pitch_of(a.C), Q = scales_of(a.C), Pt = pitch_of(a.R), Qt = scales_of(a.R);
+  const int kb = blockIdx.x, last_kb = (int)((P >> 7) - 1), last_rb = (int)((Pt >> 7) - 1);
+
+  // largest magnitude of each column over the tile (and the columns' sums)
+  unsigned cm[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    unsigned m = 0;
+    float s = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) { m = max(m, mag(v[h][k][j])); s += v[h][k][j]; }
+#pragma unroll
+    for (int o = 16; o <= 32; o <<= 1) {
+      m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
+      if (a.part) s += __shfl_xor(s, o, 64);
+    }
+    cm[j] = m;
+    if (i4 == 0) { cmax[wave][8 * l + j] = m; if (a.part) csum[wave][8 * l + j] = s; }
+  }
+  __syncthreads();
+  if (a.part && threadIdx.x < 128 && c0 + (int)threadIdx.x < a.C) {
+    const int t = threadIdx.x;
+    a.part[(long long)rb * a.C + c0 + t] = (csum[0][t] + csum[1][t]) + (csum[2][t] + csum[3][t]);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) cm[j] = max(max(cmax[0][8 * l + j], cmax[1][8 * l + j]), max(cmax[2][8 * l + j], cmax[3][8 * l + j]));
+  unsigned all = 0;
+  if constexpr (TILE) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) all = max(all, cm[j]);
+    all = max16(all);
+  }
+
+  // rows
+  if (a.data) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        unsigned m = all;
+        if constexpr (!TILE) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) m = max(m, mag(v[h][k][j]));
+          m = max16(m);
+        }
+        const int byte = scale_byte<FMT>(m);
+        const float f = inv_scale(byte);
+        const float (&x)[8] = v[h][k];
+        const long long r = row_of(h, k);
+        if (r < a.R) {
+          const u32x2 w = {pack4<FMT>(x[0] * f, x[1] * f, x[2] * f, x[3] * f), pack4<FMT>(x[4] * f, x[5] * f, x[6] * f, x[7] * f)};
+          *(u32x2 *)(a.data + r * P + c) = w;
+          if (l == 0) a.scale[r * Q + kb] = (uint8_t)byte;
+          if (kb == last_kb && l > 0 && kb + l < Q) a.scale[r * Q + kb + l] = 127;
+        }
+      }
+  }
+  if (!a.data_t) return;
+  // columns
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int byte = scale_byte<FMT>(TILE ? all : cm[j]);
+    const float f = inv_scale(byte);
+    const int cl = 8 * l + j;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int piece = (2 * wave + h) ^ (l & 7);                 // 16-byte piece of the column's line; (cl >> 3) & 7 = l & 7
+      img[cl * 32 + piece * 4 + i4] = pack4<FMT>(v[h][0][j] * f, v[h][1][j] * f, v[h][2][j] * f, v[h][3][j] * f);
+    }
+    if (wave == 0 && i4 == 0 && c + j < a.C) {
+      uint8_t *s = a.scale_t + (long long)(c + j) * Qt;
+      s[rb] = (uint8_t)byte;
+      if (rb == last_rb)
+        for (long long t = rb + 1; t < Qt; ++t) s[t] = 127;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int idx = threadIdx.x + 256 * q, cl = idx >> 3, piece = idx & 7;
+    if (c0 + cl < a.C)
+      *(u32x4 *)(a.data_t + (long long)(c0 + cl) * Pt + r0 + piece * 16) = *(const u32x4 *)(img + cl * 32 + (piece ^ ((cl >> 3) & 7)) * 4);
+  }
+}
+
+// out[c] = sum_b part[b][c]: 8 columns x 32 slices of b per workgroup, a fixed order
+__global__ __launch_bounds__(256) void colsum_parts_kernel(const float *part, int nparts, int C, float *out) {
+  __shared__ float red[32][9];
+  const int ci = threadIdx.x & 7, slice = threadIdx.x >> 3, c = blockIdx.x * 8 + ci;
+  float s = 0.f;
+  if (c < C) {
+#pragma unroll 8
+    for (int b = slice; b < nparts; b += 32) s += part[(long long)b * C + c];
+  }
+  red[slice][ci] = s;
+  __syncthreads();
+  if (slice == 0 && c < C) {
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) s += red[k][ci];
+    out[c] = s;
+  }
+}
+
+}  // namespace rows
+}  // namespace snipper

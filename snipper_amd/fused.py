@@ -384,6 +384,106 @@ def ln_fusable(x: torch.Tensor, norm: torch.nn.LayerNorm) -> bool:
             x.numel() < 2 ** 32)
 
 
+_ROW_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 3}      # include/snipper_fp8.h
+
+
+def _norm_rows(x: torch.Tensor, norm: torch.nn.LayerNorm, what: str):
+    """(x as [rows, C] with unit stride inside a row, row stride, gamma, beta, parameter type) of a layer norm over x's last axis."""
+    if not x.is_cuda:
+        raise RuntimeError(f"{what}: Not implemented on the CPU")
+    if x.dim() < 1 or tuple(norm.normalized_shape) != (x.shape[-1],):
+        raise ValueError(f"{what}: normalized_shape {tuple(norm.normalized_shape)} is not the last axis of {tuple(x.shape)}")
+    C = x.shape[-1]
+    if not 1 <= C <= 16384:
+        raise ValueError(f"{what}: rows of 1 to 16384 elements, got {C}")
+    if x.dtype not in _ROW_DT:
+        raise TypeError(f"{what}: float32, bfloat16 or float16, got {x.dtype}")
+    gamma, beta = norm.weight, norm.bias
+    p_dtype = x.dtype
+    for p in (gamma, beta):
+        if p is not None:
+            if p.dtype not in _ROW_DT or p.device != x.device or not p.is_contiguous():
+                raise TypeError(f"{what}: parameters are contiguous, of a floating type, on x's device")
+            p_dtype = p.dtype
+    if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
+        raise TypeError(f"{what}: weight and bias of one type")
+    x2 = x if x.dim() == 2 else x.reshape(-1, C)
+    if x2.stride(1) != 1 or (x2.shape[0] > 1 and x2.stride(0) < C):
+        x2 = x2.contiguous()
+    if x2.shape[0] >= 2 ** 31:
+        raise ValueError(f"{what}: fewer than 2^31 rows")
+    return x2, (x2.stride(0) if x2.shape[0] > 1 else C), gamma, beta, p_dtype
+
+
+def _opt(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _layer_norm_forward(x2, ld, gamma, beta, p_dtype, eps, y, stats, blocks=None, fmt=0):
+    """One launch of snipper_layernorm_forward; nothing for a matrix without rows."""
+    if x2.shape[0] == 0:
+        return
+    dev = x2.device
+    with _lib.device_guard(dev):
+        rc = _lib.load().snipper_layernorm_forward(
+            _stream(dev), x2.data_ptr(), _ROW_DT[x2.dtype], ld, _opt(gamma), _opt(beta), _ROW_DT[p_dtype], x2.shape[0], x2.shape[1],
+            float(eps), _opt(y), stats[0].data_ptr() if stats is not None else None, stats[1].data_ptr() if stats is not None else None,
+            blocks[0].data_ptr() if blocks is not None else None, blocks[1].data_ptr() if blocks is not None else None, fmt)
+    _lib.check(rc, "snipper_layernorm_forward")
+
+
+def _layer_norm_backward(g2, x2, ld, stats, gamma, p_dtype, want_dx, want_params):
+    """(dx like g2 or None, (dgamma, dbeta) or None)."""
+    R, C = g2.shape
+    dev = g2.device
+    dx = torch.empty((R, C), dtype=x2.dtype, device=dev) if want_dx else None
+    dp = torch.empty((2, C), dtype=p_dtype, device=dev) if want_params else None
+    if not want_params and (R == 0 or not want_dx):
+        return dx, dp
+    lib = _lib.load()
+    nbytes = lib.snipper_layernorm_backward_workspace_bytes(R, C) if want_params else 0
+    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=dev) if nbytes else None
+    with _lib.device_guard(dev):
+        rc = lib.snipper_layernorm_backward(
+            _stream(dev), g2.data_ptr(), x2.data_ptr(), _ROW_DT[x2.dtype], ld, stats[0].data_ptr(), stats[1].data_ptr(), _opt(gamma),
+            _ROW_DT[p_dtype], R, C, _opt(dx), dp[0].data_ptr() if want_params else None, dp[1].data_ptr() if want_params else None,
+            _opt(ws), nbytes)
+    _lib.check(rc, "snipper_layernorm_backward")
+    return dx, dp
+
+
+class LayerNormRows(Function):
+    """apply(x, gamma, beta, norm): see ``layer_norm``."""
+
+    @staticmethod
+    def forward(ctx, x, gamma, beta, norm):
+        x2, ld, gamma, beta, p_dtype = _norm_rows(x, norm, "layer_norm")
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        need = any(ctx.needs_input_grad[:3])
+        stats = torch.empty((2, x2.shape[0]), dtype=torch.float32, device=x.device) if need else None
+        _layer_norm_forward(x2, ld, gamma, beta, p_dtype, norm.eps, y, stats)
+        ctx.p_dtype, ctx.ld = p_dtype, ld
+        ctx.save_for_backward(x2, stats, gamma)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x2, stats, gamma = ctx.saved_tensors
+        wx, wg, wb = ctx.needs_input_grad[:3]
+        g2 = g.to(x2.dtype).contiguous().view(x2.shape)
+        dx, dp = _layer_norm_backward(g2, x2, ctx.ld, stats, gamma, ctx.p_dtype, wx, wg or wb)
+        return dx.view(g.shape) if wx else None, dp[0] if wg else None, dp[1] if wb else None, None
+
+
+def layer_norm(x: torch.Tensor, norm: torch.nn.LayerNorm) -> torch.Tensor:
+    """``norm(x)`` as one launch forward and two backward (csrc/layernorm_rows.cuh), for what ``add_dropout_layer_norm`` does not
+    take: rows of any width up to 16384, any row stride, float16 beside float32 and bfloat16, an ``nn.LayerNorm`` without weight or
+    bias.  The result and dx have x's type, dgamma and dbeta the parameters' (which is x's or another of the three); statistics and
+    sums are float32, dgamma and dbeta are summed in a fixed order."""
+    return LayerNormRows.apply(x, norm.weight, norm.bias, norm)
+
+
 class InputProjTokens(Function):
     """All input projections of the model (1x1 convolution + GroupNorm per backbone level, reference
     models/model.py:62-84) followed by the flatten + concatenation of models/deformable_transformer.py:103-122, written
