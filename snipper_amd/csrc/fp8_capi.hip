@@ -61,7 +61,7 @@ int ln_bwd_blocks(int rows, int cols) {
 
 // ---- product: which kernel, and how many pieces the K axis is cut into
 struct MmPlan {
-  int kind;                  // 0 few rows, 1 tiles of 128 x 128, 2 tiles of 256 x 256
+  int kind;                  // 0 few rows, 1 tiles of 128 x 128, 2 tiles of 256 x 256, 3 B in registers
   int tiles, splits, per_split, waves, row_tiles;
 };
 MmPlan mm_plan(int M, int N, int K, bool exact) {
@@ -74,6 +74,13 @@ MmPlan mm_plan(int M, int N, int K, bool exact) {
     p.waves = std::max(1, std::min(16, steps / 4));
     return p;
   }
+  // K <= 1024: loads and stores bound such products, and the kernel with B in registers overlaps them; whole 16-byte pieces of rows
+  // only, and at least as many chunks of 64 rows as there are CUs
+  if (!exact && steps <= 8 && N % 8 == 0 && (long long)ceil_div(M, 64) * ceil_div(N, 256) >= kCUs && (long long)N * 128 <= 0x7fffffff) {
+    p.kind = 3;
+    p.tiles = std::max(1, kCUs / (8 * ceil_div(N, 256))) * 8;     // chunk lists: one workgroup per CU
+    return p;
+  }
   const long long big = (long long)ceil_div(M, 256) * ceil_div(N, 256);
   p.kind = !exact && big >= kCUs ? 2 : 1;
   const int edge = p.kind == 2 ? 256 : 128;
@@ -84,6 +91,14 @@ MmPlan mm_plan(int M, int N, int K, bool exact) {
     p.splits = ceil_div(steps, p.per_split);
   }
   return p;
+}
+
+template <int FA, int FB, int KS = 1>
+void launch_stationary(const MmArgs &a, int n_series, hipStream_t st) {
+  if constexpr (KS < 8) {
+    if (a.steps > KS) return launch_stationary<FA, FB, KS + 1>(a, n_series, st);
+  }
+  hipLaunchKernelGGL((mm_stationary_kernel<FA, FB, KS>), dim3(n_series * ceil_div(a.N, 256)), dim3(512), 0, st, a, n_series);
 }
 
 }  // namespace
@@ -165,7 +180,10 @@ int snipper_fp8_matmul(void *stream, const uint8_t *A, const uint8_t *a_scale, i
           else hipLaunchKernelGGL((mm_rows_kernel<FA, FB, E, 4>), grid, block, lds, st, a);
         } else if (p.kind == 1) {
           hipLaunchKernelGGL((mm_tile_kernel<FA, FB, E, 2, 2, 4, 4>), dim3(p.tiles, p.splits), dim3(256), 0, st, a);
-        } else if constexpr (!E) {
+        } else if constexpr (E) {
+        } else if (p.kind == 3) {
+          launch_stationary<FA, FB>(a, p.tiles, st);
+        } else {
           hipLaunchKernelGGL((mm_tile_kernel<FA, FB, false, 2, 4, 8, 4>), dim3(p.tiles, p.splits), dim3(512), 0, st, a);
         }
       };

@@ -10,8 +10,9 @@
 // of a float32 one.  EXACT kernels therefore widen the operands to bfloat16 with their scales -- 4 bits and a power of two fit
 // exactly -- and use v_mfma_f32_16x16x32_bf16 (1e-7), at a quarter of the rate.
 //
-// Rows of n are the first operand and rows of m the second, so that a lane holds four consecutive columns of one row of the result.
+// Rows of n are the first operand and rows of m the second, so that a lane holds consecutive columns of one row of the result.
 #pragma once
+#include <utility>
 #include "rows_common.cuh"
 
 namespace snipper {
@@ -33,33 +34,48 @@ struct MmArgs {
   int splits, per_split;                     // K steps of a split (a multiple of 4)
 };
 
-// four elements of a row of the result: columns n .. n + 3
-__device__ __forceinline__ void mm_store4(const MmArgs &a, long long m, int n, f32x4 v) {
+__device__ __forceinline__ uint16_t mm_half(float v, int dt) {
+  return dt == kBF16 ? __builtin_bit_cast(uint16_t, (bf16_t)v) : __builtin_bit_cast(uint16_t, (f16_t)v);
+}
+// W elements of a row of the result: columns n .. n + W - 1
+template <int W>
+__device__ __forceinline__ void mm_store(const MmArgs &a, long long m, int n, const float (&acc)[W]) {
   const int cnt = a.N - n;
   if (cnt <= 0) return;
+  float v[W];
+#pragma unroll
+  for (int t = 0; t < W; ++t) v[t] = acc[t];
   if (a.bias) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) v[t] += t < cnt ? load_param(a.bias, a.bias_dt, n + t) : 0.f;
+    for (int t = 0; t < W; ++t) v[t] += t < cnt ? load_param(a.bias, a.bias_dt, n + t) : 0.f;
   }
   if (a.relu) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) v[t] = v[t] < 0.f ? 0.f : v[t];      // (a NaN stays one)
+    for (int t = 0; t < W; ++t) v[t] = v[t] < 0.f ? 0.f : v[t];      // (a NaN stays one)
   }
   const long long at = m * a.N + n;
   if (a.out_dt == kF32) {
     float *p = (float *)a.out + at;
-    if (cnt >= 4) __builtin_memcpy(p, &v, 16);
-    else for (int t = 0; t < cnt; ++t) p[t] = v[t];
-  } else {
-    uint16_t h[4];
+    if (cnt >= W) __builtin_memcpy(p, v, 4 * W);
+    else {
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-      h[t] = a.out_dt == kBF16 ? __builtin_bit_cast(uint16_t, (bf16_t)v[t]) : __builtin_bit_cast(uint16_t, (f16_t)v[t]);
+      for (int t = 0; t < W; ++t) if (t < cnt) p[t] = v[t];
+    }
+  } else {
+    uint16_t h[W];
+#pragma unroll
+    for (int t = 0; t < W; ++t) h[t] = mm_half(v[t], a.out_dt);
     uint16_t *p = (uint16_t *)a.out + at;
-    if (cnt >= 4) __builtin_memcpy(p, h, 8);
-    else for (int t = 0; t < cnt; ++t) p[t] = h[t];
+    if (cnt >= W) __builtin_memcpy(p, h, 2 * W);
+    else {
+#pragma unroll
+      for (int t = 0; t < W; ++t) if (t < cnt) p[t] = h[t];
+    }
   }
 }
+// Which row of B a lane holds in operand j of a pair (j even, j + 1): with these the two 16 x 16 results of a pair give a lane eight
+// consecutive columns of a row, 16 bytes of a 16-bit result, and a wave's store whole 64-byte pieces.
+__device__ __forceinline__ int mm_pair_row(int j, int r) { return 32 * (j >> 1) + 8 * (r >> 2) + 4 * (j & 1) + (r & 3); }
 
 // 8 bytes -> 8 bfloat16, times 2^(byte - 127)
 template <int FMT>
@@ -114,8 +130,8 @@ __device__ __forceinline__ f32x4 mm_step(const Operand<FB, true> &b, const Opera
 
 // ---- tiles -----------------------------------------------------------------------------------------------------------
 // A workgroup of WM x WN waves makes a (16 TM WM) x (16 TN WN) tile; a K step of 128 is one byte-row of 128 per row of either side.
-// Rows go to LDS by DMA in 16-byte pieces, piece c of row r at place c ^ (r & 7), so that the 16 rows of an operand are read without
-// bank conflicts; two buffers, one barrier a step.  The scale words of four K steps come the same way (plain loads of them would make
+// Rows go to LDS by DMA in 16-byte pieces, piece c of row r at place c ^ key(r), so that the 16 rows of an operand are read without
+// bank conflicts (A: consecutive rows, key = r & 7; B: rows of mm_pair_row, key = bits 0, 1 and 3 of r); two buffers, one barrier a step.  The scale words of four K steps come the same way (plain loads of them would make
 // the compiler wait for the DMAs issued after them).
 template <int FA, int FB, bool EXACT, int WM, int WN, int TM, int TN>
 __global__ __launch_bounds__(64 * WM * WN) void mm_tile_kernel(MmArgs a) {
@@ -148,7 +164,8 @@ __global__ __launch_bounds__(64 * WM * WN) void mm_tile_kernel(MmArgs a) {
       const int q = wave + kWaves * d;                          // rows 8 q .. 8 q + 7 of the buffer: first A's, then B's
       const bool is_a = q < BM / 8;
       const int row = (is_a ? q : q - BM / 8) * 8 + (lane >> 3);
-      const unsigned voff = (unsigned)row * (unsigned)P + (unsigned)(((lane & 7) ^ (lane >> 3)) * 16);
+      const int key = is_a ? lane >> 3 : ((lane >> 3) & 3) | ((q & 1) << 2);
+      const unsigned voff = (unsigned)row * (unsigned)P + (unsigned)(((lane & 7) ^ key) * 16);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(is_a ? asrc : bsrc, (__attribute__((address_space(3))) void *)(smem + buf * kBuf + q * 1024), 16,
                                                voff, kt * 128, 0, 0);
     }
@@ -171,10 +188,11 @@ __global__ __launch_bounds__(64 * WM * WN) void mm_tile_kernel(MmArgs a) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  auto read_frag = [&](const unsigned char *rowp, i32x4 &lo, i32x4 &hi) {
-    lo = *(const i32x4 *)(rowp + (((2 * g) ^ (r & 7)) * 16));
-    hi = *(const i32x4 *)(rowp + (((2 * g + 1) ^ (r & 7)) * 16));
+  auto read_frag = [&](const unsigned char *rowp, int key, i32x4 &lo, i32x4 &hi) {
+    lo = *(const i32x4 *)(rowp + (((2 * g) ^ key) * 16));
+    hi = *(const i32x4 *)(rowp + (((2 * g + 1) ^ key) * 16));
   };
+  const int key_b = (r & 3) | (r & 4);                          // bit 3 of mm_pair_row(., r) is bit 2 of r
   auto step = [&](auto sel_c, int kt) {
     constexpr int SEL = decltype(sel_c)::value;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -189,20 +207,20 @@ __global__ __launch_bounds__(64 * WM * WN) void mm_tile_kernel(MmArgs a) {
 #pragma unroll
       for (int i = 0; i < TM; ++i) sa[i] = sc[(wm * TM + i) * 16 + r];
 #pragma unroll
-      for (int j = 0; j < TN; ++j) sb[j] = sc[BM + (wn * TN + j) * 16 + r];
+      for (int j = 0; j < TN; ++j) sb[j] = sc[BM + wn * TN * 16 + mm_pair_row(j, r)];
     }
     const unsigned char *base = smem + (kt & 1) * kBuf;
     Operand<FB, EXACT> b[TN];
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       i32x4 lo, hi;
-      read_frag(base + (BM + (wn * TN + j) * 16 + r) * 128, lo, hi);
+      read_frag(base + (BM + wn * TN * 16 + mm_pair_row(j, r)) * 128, key_b, lo, hi);
       b[j].set(lo, hi, sb[j], SEL);
     }
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       i32x4 lo, hi;
-      read_frag(base + ((wm * TM + i) * 16 + r) * 128, lo, hi);
+      read_frag(base + ((wm * TM + i) * 16 + r) * 128, r & 7, lo, hi);
       Operand<FA, EXACT> x;
       x.set(lo, hi, sa[i], SEL);
 #pragma unroll
@@ -220,22 +238,19 @@ __global__ __launch_bounds__(64 * WM * WN) void mm_tile_kernel(MmArgs a) {
     if (kt + 3 < k_end) step(std::integral_constant<int, 3>{}, kt + 3);
   }
 
-  // a lane's four consecutive columns of row (l & 15) of each 16 x 16 piece
+  // a lane's eight consecutive columns of row (l & 15) of each pair of 16 x 16 pieces
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
     const long long m = m0 + (wm * TM + i) * 16 + r;
     if (m >= a.M) continue;
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int n = n0 + (wn * TN + j) * 16 + 4 * g;
-      if (a.part) {
-        float *p = a.part + ((long long)blockIdx.y * a.M + m) * a.N + n;
+    for (int j = 0; j < TN; j += 2) {
+      const int n = n0 + wn * TN * 16 + j * 16 + 8 * g;
+      float v[8];
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (n + q < a.N) p[q] = acc[i][j][q];
-      } else {
-        mm_store4(a, m, n, acc[i][j]);
-      }
+      for (int q = 0; q < 4; ++q) { v[q] = acc[i][j][q]; v[4 + q] = acc[i][j + 1][q]; }
+      if (a.part) store8(a.part + ((long long)blockIdx.y * a.M + m) * a.N + n, a.N - n, v);
+      else mm_store(a, m, n, v);
     }
   }
 }
@@ -255,8 +270,140 @@ __global__ __launch_bounds__(256) void mm_join_kernel(MmArgs a) {
       else for (int t = 0; t < cnt; ++t) w[t] = p[t];
       v += w;
     }
-    mm_store4(a, m, n, v);
+    const float o[4] = {v[0], v[1], v[2], v[3]};
+    mm_store(a, m, n, o);
   }
+}
+
+// a value that has been loaded: the wait for its load is placed here
+template <typename T>
+__device__ __forceinline__ void settle(T &x) { asm volatile("" : "+v"(x)); }
+// all but the last N vector memory instructions of this wave are done
+template <int N>
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+// f(0), f(1), ... with constants
+template <typename F, int... K>
+__device__ __forceinline__ void each_step(F &&f, std::integer_sequence<int, K...>) { (f(std::integral_constant<int, K>{}), ...); }
+
+// the loads of a chunk of 64 rows and of its scale words, KS + ceil(KS / 4) instructions of every wave; behind the last chunk the range
+// is empty and nothing arrives
+template <int KS>
+__device__ __forceinline__ void issue_chunk(const MmArgs &a, unsigned char *slot, const unsigned *voff, int chunk, int wave, int lane) {
+  constexpr int PB = KS * 128, QB = (KS + 3) / 4 * 4;
+  const int rows = max(0, min(64, a.M - chunk * 64));
+  const long long first = rows > 0 ? (long long)chunk * 64 : 0;
+  const __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(a.A + first * PB), 0, rows * PB, 0x00020000);
+  const __amdgpu_buffer_rsrc_t ssrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(a.sA + first * QB), 0, rows * QB, 0x00020000);
+#pragma unroll
+  for (int d = 0; d < KS; ++d)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void *)(slot + (wave * KS + d) * 1024), 16, voff[d], 0, 0, 0);
+#pragma unroll
+  for (int d = 0; d < QB / 4; ++d)                              // (every wave the same words: the counts stay equal)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(ssrc, (__attribute__((address_space(3))) void *)(slot + 64 * PB + d * 256), 4,
+                                             (unsigned)(d * 64 + lane) * 4, 0, 0, 0);
+}
+
+// ---- short rows, many of them ----------------------------------------------------------------------------------------
+// K <= 128 KS: B stays in registers.  Each of the eight waves holds 32 columns (two operands of KS steps, 16 KS registers), a workgroup
+// 256; the rows of A stream past in chunks of 64 through an LDS ring filled by DMA, and one persistent workgroup per CU walks over
+// chunks.  A tile kernel of such shapes spends its time filling and draining: its two or three K steps do not cover the latency of
+// their loads, nor the stores of the tile before.  Here loads run S - 1 chunks ahead across the stores; the counted waits rely on every
+// wave issuing the same number of memory instructions per chunk, so rows and columns past the end go through the buffers' range
+// checks.  The workgroups that share a chunk sit on one XCD: A comes from HBM once.
+template <int FA, int FB, int KS>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void mm_stationary_kernel(MmArgs a, int n_series) {
+  constexpr int ROWS = 64, PB = KS * 128, S = KS <= 4 ? 4 : KS <= 6 ? 3 : 2, QW = (KS + 3) / 4, kChunk = ROWS * PB, kScl = ROWS * QW * 4;
+  constexpr int kLoads = KS + QW, kStores = 4;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[S * (kChunk + kScl)];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const int ncb = (a.N + 255) >> 8, per_group = 8 * ncb;
+  const int grp = blockIdx.x / per_group, within = blockIdx.x - grp * per_group;
+  const int series = grp * 8 + (within & 7), n0 = (within >> 3) * 256 + wave * 32;
+  const int chunks = (a.M + ROWS - 1) / ROWS;
+  const int iters = series < chunks ? (chunks - series + n_series - 1) / n_series : 0;
+  if (iters == 0) return;                                       // (the whole workgroup)
+
+  // piece c of row `row` of a chunk lies at place c ^ (row & 7) of its 128 bytes; a wave's instruction moves 64 pieces
+  unsigned voff[KS];
+#pragma unroll
+  for (int d = 0; d < KS; ++d) {
+    const int p = (wave * KS + d) * 64 + lane, row = p / (8 * KS), c = p - row * (8 * KS);
+    voff[d] = row * PB + ((c & ~7) | ((c ^ row) & 7)) * 16;
+  }
+  i32x8 b[2][KS];
+  int sb[2][QW];
+  float bias[8];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const long long n = min(n0 + mm_pair_row(j, r), a.N - 1);
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const i32x4 lo = *(const i32x4 *)(a.B + n * PB + k * 128 + g * 32), hi = *(const i32x4 *)(a.B + n * PB + k * 128 + g * 32 + 16);
+      b[j][k] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+#pragma unroll
+    for (int q = 0; q < QW; ++q) sb[j][q] = *(const int *)(a.sB + n * QW * 4 + q * 4);
+  }
+  load_param8(a.bias, a.bias_dt, n0 + 8 * g, a.N - (n0 + 8 * g), 0.f, bias);
+  // the loads above are waited for here, not at their first use in the loop (where the wait would drain the ring every time)
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+#pragma unroll
+    for (int k = 0; k < KS; ++k) settle(b[j][k]);
+#pragma unroll
+    for (int q = 0; q < QW; ++q) settle(sb[j][q]);
+  }
+#pragma unroll
+  for (int t = 0; t < 8; ++t) settle(bias[t]);
+#pragma unroll
+  for (int it = 0; it < S - 1; ++it) issue_chunk<KS>(a, smem + it * (kChunk + kScl), voff, it < iters ? series + it * n_series : chunks, wave, lane);
+
+  for (int it = 0; it < iters; ++it) {
+    // chunk `it` has come when all but the instructions behind its loads are done: S - 2 chunks of loads and (once the pipe is
+    // full) S - 1 chunks of stores
+    if (it < S - 1) wait_loads<(S - 2) * kLoads>();
+    else wait_loads<(S - 2) * kLoads + (S - 1) * kStores>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    const int ahead = it + S - 1;                               // into the slot that every wave has left
+    issue_chunk<KS>(a, smem + (ahead % S) * (kChunk + kScl), voff, ahead < iters ? series + ahead * n_series : chunks, wave, lane);
+    const unsigned char *slot = smem + (it % S) * (kChunk + kScl);
+    const int *scl = (const int *)(slot + kChunk);
+    const int chunk = series + it * n_series;
+    const int rows = min(ROWS, a.M - chunk * ROWS);
+    const __amdgpu_buffer_rsrc_t dst = __builtin_amdgcn_make_buffer_rsrc((uint16_t *)a.out + (long long)chunk * ROWS * a.N, 0, rows * a.N * 2, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = 16 * i + r;
+      f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+      int sa[QW];
+#pragma unroll
+      for (int q = 0; q < QW; ++q) sa[q] = scl[row * QW + q];
+      each_step([&](auto step) {
+        constexpr int K = decltype(step)::value;
+        const unsigned char *at = slot + row * PB + K * 128;
+        Operand<FA, false> x;
+        x.set(*(const i32x4 *)(at + (((2 * g) ^ (r & 7)) * 16)), *(const i32x4 *)(at + (((2 * g + 1) ^ (r & 7)) * 16)), 0, 0);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[j] = mm_step<FB, FA, K & 3>(Operand<FB, false>{b[j][K]}, x, acc[j], sb[j][K >> 2], sa[K >> 2]);
+      }, std::make_integer_sequence<int, KS>{});
+      uint16_t h[8];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        float v = acc[t >> 2][t & 3] + bias[t];
+        v = a.relu && v < 0.f ? 0.f : v;
+        h[t] = mm_half(v, a.out_dt);
+      }
+      u32x4 w;
+      __builtin_memcpy(&w, h, 16);
+      const int n = n0 + 8 * g;
+      __builtin_amdgcn_raw_buffer_store_b128(w, dst, n < a.N ? (unsigned)row * (unsigned)a.N * 2u + (unsigned)n * 2u : 0x80000000u, 0, 0);
+    }
+  }
+  wait_loads<0>();                                              // (the empty loads behind the last chunk)
 }
 
 // ---- few rows -----------------------------------------------------------------------------------------------------------
@@ -301,7 +448,8 @@ __global__ __launch_bounds__(1024) void mm_rows_kernel(MmArgs a) {
     f32x4 v = red[i * 64 + lane];
     for (int w = 1; w < W; ++w) v += red[(w * T + i) * 64 + lane];
     const long long m = m0 + 16 * i + r;
-    if (m < a.M) mm_store4(a, m, n0 + 4 * g, v);
+    const float o[4] = {v[0], v[1], v[2], v[3]};
+    if (m < a.M) mm_store(a, m, n0 + 4 * g, o);
   }
 }
 
