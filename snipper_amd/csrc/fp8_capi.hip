@@ -82,7 +82,7 @@ MmPlan mm_plan(int M, int N, int K, bool exact) {
     return p;
   }
   const long long big = (long long)ceil_div(M, 256) * ceil_div(N, 256);
-  p.kind = !exact && big >= kCUs ? 2 : 1;
+  p.kind = !exact && M >= 256 && N >= 256 && big >= kCUs ? 2 : 1;
   const int edge = p.kind == 2 ? 256 : 128;
   p.tiles = ceil_div(M, edge) * ceil_div(N, edge);
   if (p.tiles < 2 * kCUs && steps >= 8) {
@@ -179,12 +179,12 @@ int snipper_fp8_matmul(void *stream, const uint8_t *A, const uint8_t *a_scale, i
           else if (p.row_tiles == 2) hipLaunchKernelGGL((mm_rows_kernel<FA, FB, E, 2>), grid, block, lds, st, a);
           else hipLaunchKernelGGL((mm_rows_kernel<FA, FB, E, 4>), grid, block, lds, st, a);
         } else if (p.kind == 1) {
-          hipLaunchKernelGGL((mm_tile_kernel<FA, FB, E, 2, 2, 4, 4>), dim3(p.tiles, p.splits), dim3(256), 0, st, a);
+          hipLaunchKernelGGL((mm_tile_kernel<FA, FB, E, 2, 2, 4, 4, false>), dim3(p.tiles, p.splits), dim3(256), 0, st, a);
         } else if constexpr (E) {
         } else if (p.kind == 3) {
           launch_stationary<FA, FB>(a, p.tiles, st);
         } else {
-          hipLaunchKernelGGL((mm_tile_kernel<FA, FB, false, 2, 4, 8, 4>), dim3(p.tiles, p.splits), dim3(512), 0, st, a);
+          hipLaunchKernelGGL((mm_tile_kernel<FA, FB, false, 2, 4, 8, 4, true>), dim3(p.tiles, p.splits), dim3(512), 0, st, a);
         }
       };
       if (exact) go(std::true_type{});

@@ -37,21 +37,21 @@ struct MmArgs {
 __device__ __forceinline__ uint16_t mm_half(float v, int dt) {
   return dt == kBF16 ? __builtin_bit_cast(uint16_t, (bf16_t)v) : __builtin_bit_cast(uint16_t, (f16_t)v);
 }
+template <int W>
+__device__ __forceinline__ void mm_bias(const MmArgs &a, int n, float (&v)[W]) {       // of columns n .. n + W - 1, 0 where there is none
+#pragma unroll
+  for (int t = 0; t < W; ++t) v[t] = a.bias && n + t < a.N ? load_param(a.bias, a.bias_dt, n + t) : 0.f;
+}
 // W elements of a row of the result: columns n .. n + W - 1
 template <int W>
-__device__ __forceinline__ void mm_store(const MmArgs &a, long long m, int n, const float (&acc)[W]) {
+__device__ __forceinline__ void mm_store(const MmArgs &a, long long m, int n, const float (&acc)[W], const float (&bias)[W]) {
   const int cnt = a.N - n;
   if (cnt <= 0) return;
   float v[W];
 #pragma unroll
-  for (int t = 0; t < W; ++t) v[t] = acc[t];
-  if (a.bias) {
-#pragma unroll
-    for (int t = 0; t < W; ++t) v[t] += t < cnt ? load_param(a.bias, a.bias_dt, n + t) : 0.f;
-  }
-  if (a.relu) {
-#pragma unroll
-    for (int t = 0; t < W; ++t) v[t] = v[t] < 0.f ? 0.f : v[t];      // (a NaN stays one)
+  for (int t = 0; t < W; ++t) {
+    v[t] = acc[t] + bias[t];
+    v[t] = a.relu && v[t] < 0.f ? 0.f : v[t];                         // (a NaN stays one)
   }
   const long long at = m * a.N + n;
   if (a.out_dt == kF32) {
@@ -128,12 +128,32 @@ __device__ __forceinline__ f32x4 mm_step(const Operand<FB, true> &b, const Opera
   return acc;
 }
 
+// a value that has been loaded: the wait for its load is placed here
+template <typename T>
+__device__ __forceinline__ void settle(T &x) { asm volatile("" : "+v"(x)); }
+// 16 (4) bytes per lane from base + voff + soff to LDS, lane after lane; for offsets voff >= range zeros
+__device__ __forceinline__ void dma16(const uint8_t *base, int range, unsigned char *lds, unsigned voff, unsigned soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, range, 0x00020000),
+                                           (__attribute__((address_space(3))) void *)lds, 16, voff, soff, 0, 0);
+}
+__device__ __forceinline__ void dma4(const uint8_t *base, int range, unsigned char *lds, unsigned voff, unsigned soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, range, 0x00020000),
+                                           (__attribute__((address_space(3))) void *)lds, 4, voff, soff, 0, 0);
+}
+// all but the last N vector memory instructions of this wave are done
+template <int N>
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
 // ---- tiles -----------------------------------------------------------------------------------------------------------
 // A workgroup of WM x WN waves makes a (16 TM WM) x (16 TN WN) tile; a K step of 128 is one byte-row of 128 per row of either side.
-// Rows go to LDS by DMA in 16-byte pieces, piece c of row r at place c ^ key(r), so that the 16 rows of an operand are read without
-// bank conflicts (A: consecutive rows, key = r & 7; B: rows of mm_pair_row, key = bits 0, 1 and 3 of r); two buffers, one barrier a step.  The scale words of four K steps come the same way (plain loads of them would make
+// Rows go to LDS by DMA in 16-byte pieces, piece c of row r at place c ^ key(r), and a lane takes pieces g and g + 4 of its row (both
+// sides alike), so that reads are free of bank conflicts: a 16-byte read serves lanes 0-3, 12-15, 20-27, then 4-11, 16-19, 28-31, then
+// the same of the upper half, 256 bytes each (counted; keys that suit groups of 8 or 16 neighbours cost twice the clocks).  A:
+// consecutive rows, key = r & 7; B: rows of mm_pair_row, key = bits 0, 1 and 3 of r; two buffers, one barrier a step.  The scale words of four K steps come the same way (plain loads of them would make
 // the compiler wait for the DMAs issued after them).
-template <int FA, int FB, bool EXACT, int WM, int WN, int TM, int TN>
+// INWARD (M >= BM, N >= BN): the last tile of an edge is moved inwards, and two workgroups store the same values; rows need no range
+// checks then, and their addresses one register a side instead of one for each load.
+template <int FA, int FB, bool EXACT, int WM, int WN, int TM, int TN, bool INWARD>
 __global__ __launch_bounds__(64 * WM * WN) void mm_tile_kernel(MmArgs a) {
   constexpr int kWaves = WM * WN, BM = 16 * TM * WM, BN = 16 * TN * WN, kBuf = (BM + BN) * 128, kScl = (BM + BN) * 4;
   static_assert((BM + BN) % (8 * kWaves) == 0 && BM % 8 == 0, "whole DMA instructions of 8 rows");
@@ -150,35 +170,33 @@ __global__ __launch_bounds__(64 * WM * WN) void mm_tile_kernel(MmArgs a) {
   const int id = blockIdx.x, per = tiles >> 3, rem = tiles & 7, xcd = id & 7;
   const int t = xcd * per + (xcd < rem ? xcd : rem) + (id >> 3);
   const int band = t / (8 * tn_n), in_band = t - band * 8 * tn_n, bh = min(8, tm_n - band * 8);
-  const int m0 = (band * 8 + in_band % bh) * BM, n0 = (in_band / bh) * BN;
+  int m0 = (band * 8 + in_band % bh) * BM, n0 = (in_band / bh) * BN;
+  if constexpr (INWARD) { m0 = min(m0, a.M - BM); n0 = min(n0, a.N - BN); }
 
   const long long P = (long long)a.steps * 128, Q = (long long)((a.steps + 3) >> 2) * 4;
   const int k_begin = blockIdx.y * a.per_split, k_end = min(a.steps, k_begin + a.per_split);
 
   const int rows_a = min(BM, a.M - m0), rows_b = min(BN, a.N - n0);
-  const __amdgpu_buffer_rsrc_t asrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(a.A + m0 * P), 0, (int)(rows_a * P), 0x00020000);
-  const __amdgpu_buffer_rsrc_t bsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(a.B + n0 * P), 0, (int)(rows_b * P), 0x00020000);
+  static_assert((BM / 8) % kWaves == 0 && kWaves % 2 == 0, "an instruction's side is known at compile time, its parity the wave's");
+  const unsigned key_a = lane >> 3, key_w = ((lane >> 3) & 3) | ((wave & 1) << 2);
+  const unsigned va = (8 * wave + (lane >> 3)) * (unsigned)P + ((lane & 7) ^ key_a) * 16, vb = (8 * wave + (lane >> 3)) * (unsigned)P + ((lane & 7) ^ key_w) * 16;
   auto issue = [&](int kt, int buf) {
 #pragma unroll
     for (int d = 0; d < kDma; ++d) {
-      const int q = wave + kWaves * d;                          // rows 8 q .. 8 q + 7 of the buffer: first A's, then B's
-      const bool is_a = q < BM / 8;
-      const int row = (is_a ? q : q - BM / 8) * 8 + (lane >> 3);
-      const int key = is_a ? lane >> 3 : ((lane >> 3) & 3) | ((q & 1) << 2);
-      const unsigned voff = (unsigned)row * (unsigned)P + (unsigned)(((lane & 7) ^ key) * 16);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(is_a ? asrc : bsrc, (__attribute__((address_space(3))) void *)(smem + buf * kBuf + q * 1024), 16,
-                                               voff, kt * 128, 0, 0);
+      constexpr int kA = BM / 8 / kWaves;
+      const bool is_a = d < kA;                                 // 8 rows of A, or of B, behind them
+      const unsigned rows_on = (unsigned)(is_a ? d : d - kA) * (8u * kWaves) * (unsigned)P;
+      dma16(is_a ? a.A + m0 * P : a.B + n0 * P, (int)((is_a ? rows_a : rows_b) * P), smem + buf * kBuf + (wave + kWaves * d) * 1024,
+            (is_a ? va : vb) + (INWARD ? 0u : rows_on), kt * 128u + (INWARD ? rows_on : 0u));
     }
   };
   // scale words of K steps 4 kg .. 4 kg + 3, rows as above
-  const __amdgpu_buffer_rsrc_t asc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(a.sA + m0 * Q), 0, (int)(rows_a * Q), 0x00020000);
-  const __amdgpu_buffer_rsrc_t bsc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(a.sB + n0 * Q), 0, (int)(rows_b * Q), 0x00020000);
   auto issue_scales = [&](int kg) {
     if (wave < (BM + BN) / 64) {
       const bool is_a = wave < BM / 64;
       const int row = (is_a ? wave : wave - BM / 64) * 64 + lane;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(is_a ? asc : bsc, (__attribute__((address_space(3))) void *)(smem + 2 * kBuf + (kg & 1) * kScl + wave * 256),
-                                               4, (unsigned)row * (unsigned)Q, kg * 4, 0, 0);
+      dma4(is_a ? a.sA + m0 * Q : a.sB + n0 * Q, (int)((is_a ? rows_a : rows_b) * Q), smem + 2 * kBuf + (kg & 1) * kScl + wave * 256,
+           (unsigned)row * (unsigned)Q, kg * 4);
     }
   };
   int sa[TM], sb[TN];
@@ -189,8 +207,8 @@ __global__ __launch_bounds__(64 * WM * WN) void mm_tile_kernel(MmArgs a) {
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   auto read_frag = [&](const unsigned char *rowp, int key, i32x4 &lo, i32x4 &hi) {
-    lo = *(const i32x4 *)(rowp + (((2 * g) ^ key) * 16));
-    hi = *(const i32x4 *)(rowp + (((2 * g + 1) ^ key) * 16));
+    lo = *(const i32x4 *)(rowp + ((g ^ key) * 16));
+    hi = *(const i32x4 *)(rowp + (((g + 4) ^ key) * 16));
   };
   const int key_b = (r & 3) | (r & 4);                          // bit 3 of mm_pair_row(., r) is bit 2 of r
   auto step = [&](auto sel_c, int kt) {
@@ -240,17 +258,19 @@ __global__ __launch_bounds__(64 * WM * WN) void mm_tile_kernel(MmArgs a) {
 
   // a lane's eight consecutive columns of row (l & 15) of each pair of 16 x 16 pieces
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const long long m = m0 + (wm * TM + i) * 16 + r;
-    if (m >= a.M) continue;
+  for (int j = 0; j < TN; j += 2) {
+    const int n = n0 + wn * TN * 16 + j * 16 + 8 * g;
+    float bias[8];
+    if (!a.part) mm_bias(a, n, bias);
 #pragma unroll
-    for (int j = 0; j < TN; j += 2) {
-      const int n = n0 + wn * TN * 16 + j * 16 + 8 * g;
+    for (int i = 0; i < TM; ++i) {
+      const long long m = m0 + (wm * TM + i) * 16 + r;
+      if (m >= a.M) continue;
       float v[8];
 #pragma unroll
       for (int q = 0; q < 4; ++q) { v[q] = acc[i][j][q]; v[4 + q] = acc[i][j + 1][q]; }
       if (a.part) store8(a.part + ((long long)blockIdx.y * a.M + m) * a.N + n, a.N - n, v);
-      else mm_store(a, m, n, v);
+      else mm_store(a, m, n, v, bias);
     }
   }
 }
@@ -271,37 +291,28 @@ __global__ __launch_bounds__(256) void mm_join_kernel(MmArgs a) {
       v += w;
     }
     const float o[4] = {v[0], v[1], v[2], v[3]};
-    mm_store(a, m, n, o);
+    float bias[4];
+    mm_bias(a, n, bias);
+    mm_store(a, m, n, o, bias);
   }
 }
-
-// a value that has been loaded: the wait for its load is placed here
-template <typename T>
-__device__ __forceinline__ void settle(T &x) { asm volatile("" : "+v"(x)); }
-// all but the last N vector memory instructions of this wave are done
-template <int N>
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
 // f(0), f(1), ... with constants
 template <typename F, int... K>
 __device__ __forceinline__ void each_step(F &&f, std::integer_sequence<int, K...>) { (f(std::integral_constant<int, K>{}), ...); }
 
 // the loads of a chunk of 64 rows and of its scale words, KS + ceil(KS / 4) instructions of every wave; behind the last chunk the range
-// is empty and nothing arrives
+// is empty: zeros for a slot that nobody reads
 template <int KS>
 __device__ __forceinline__ void issue_chunk(const MmArgs &a, unsigned char *slot, const unsigned *voff, int chunk, int wave, int lane) {
   constexpr int PB = KS * 128, QB = (KS + 3) / 4 * 4;
   const int rows = max(0, min(64, a.M - chunk * 64));
   const long long first = rows > 0 ? (long long)chunk * 64 : 0;
-  const __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(a.A + first * PB), 0, rows * PB, 0x00020000);
-  const __amdgpu_buffer_rsrc_t ssrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(a.sA + first * QB), 0, rows * QB, 0x00020000);
 #pragma unroll
-  for (int d = 0; d < KS; ++d)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void *)(slot + (wave * KS + d) * 1024), 16, voff[d], 0, 0, 0);
+  for (int d = 0; d < KS; ++d) dma16(a.A + first * PB, rows * PB, slot + (wave * KS + d) * 1024, voff[d], 0);
 #pragma unroll
   for (int d = 0; d < QB / 4; ++d)                              // (every wave the same words: the counts stay equal)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(ssrc, (__attribute__((address_space(3))) void *)(slot + 64 * PB + d * 256), 4,
-                                             (unsigned)(d * 64 + lane) * 4, 0, 0, 0);
+    dma4(a.sA + first * QB, rows * QB, slot + 64 * PB + d * 256, (unsigned)(d * 64 + lane) * 4, 0);
 }
 
 // ---- short rows, many of them ----------------------------------------------------------------------------------------
@@ -326,12 +337,13 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int iters = series < chunks ? (chunks - series + n_series - 1) / n_series : 0;
   if (iters == 0) return;                                       // (the whole workgroup)
 
-  // piece c of row `row` of a chunk lies at place c ^ (row & 7) of its 128 bytes; a wave's instruction moves 64 pieces
+  // piece c of row `row` of a chunk lies at place c ^ (row & 7) of its 128 bytes, and where a row is a multiple of 256 bytes the odd
+  // ones have neighbouring 128s swapped (see mm_tile_kernel on bank conflicts); a wave's instruction moves 64 pieces
   unsigned voff[KS];
 #pragma unroll
   for (int d = 0; d < KS; ++d) {
     const int p = (wave * KS + d) * 64 + lane, row = p / (8 * KS), c = p - row * (8 * KS);
-    voff[d] = row * PB + ((c & ~7) | ((c ^ row) & 7)) * 16;
+    voff[d] = row * PB + ((((c >> 3) ^ (KS % 2 ? 0 : row & 1)) << 3) | ((c ^ row) & 7)) * 16;
   }
   i32x8 b[2][KS];
   int sb[2][QW];
@@ -341,7 +353,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const long long n = min(n0 + mm_pair_row(j, r), a.N - 1);
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
-      const i32x4 lo = *(const i32x4 *)(a.B + n * PB + k * 128 + g * 32), hi = *(const i32x4 *)(a.B + n * PB + k * 128 + g * 32 + 16);
+      const i32x4 lo = *(const i32x4 *)(a.B + n * PB + k * 128 + g * 16), hi = *(const i32x4 *)(a.B + n * PB + k * 128 + g * 16 + 64);
       b[j][k] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
 #pragma unroll
@@ -384,9 +396,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       for (int q = 0; q < QW; ++q) sa[q] = scl[row * QW + q];
       each_step([&](auto step) {
         constexpr int K = decltype(step)::value;
-        const unsigned char *at = slot + row * PB + K * 128;
+        const unsigned char *at = slot + row * PB + (KS % 2 ? K : K ^ (r & 1)) * 128;
         Operand<FA, false> x;
-        x.set(*(const i32x4 *)(at + (((2 * g) ^ (r & 7)) * 16)), *(const i32x4 *)(at + (((2 * g + 1) ^ (r & 7)) * 16)), 0, 0);
+        x.set(*(const i32x4 *)(at + ((g ^ (r & 7)) * 16)), *(const i32x4 *)(at + (((g + 4) ^ (r & 7)) * 16)), 0, 0);
 #pragma unroll
         for (int j = 0; j < 2; ++j) acc[j] = mm_step<FB, FA, K & 3>(Operand<FB, false>{b[j][K]}, x, acc[j], sb[j][K >> 2], sa[K >> 2]);
       }, std::make_integer_sequence<int, KS>{});
@@ -449,7 +461,9 @@ __global__ __launch_bounds__(1024) void mm_rows_kernel(MmArgs a) {
     for (int w = 1; w < W; ++w) v += red[(w * T + i) * 64 + lane];
     const long long m = m0 + 16 * i + r;
     const float o[4] = {v[0], v[1], v[2], v[3]};
-    if (m < a.M) mm_store(a, m, n0 + 4 * g, o);
+    float bias[4];
+    mm_bias(a, n0 + 4 * g, bias);
+    if (m < a.M) mm_store(a, m, n0 + 4 * g, o, bias);
   }
 }
 
