@@ -48,15 +48,16 @@ void with_ln_shape(int cols, F &&f) {
   if (cols <= 128) f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
   else if (cols <= 512) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
   else if (cols <= 1024) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
-  else if (cols <= 2048) f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
-  else if (cols <= 4096) f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
-  else if (cols <= 8192) f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+  else if (cols <= 2048) f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+  else if (cols <= 4096) f(integral_constant<int, 512>{}, integral_constant<int, 1>{});
+  else if (cols <= 8192) f(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
   else f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
 }
-int ln_rows_per_wg(int cols) { return cols <= 128 ? 16 : cols <= 2048 ? 4 : 1; }
-int ln_fwd_blocks(int rows, int cols) { return std::min(ceil_div(rows, ln_rows_per_wg(cols)), cols > 8192 ? 2 * kCUs : 8 * kCUs); }
+int ln_rows_per_wg(int cols) { return cols <= 128 ? 16 : cols <= 1024 ? 4 : 1; }
+int ln_wgs_per_cu(int cols) { return cols <= 2048 ? 8 : cols <= 4096 ? 4 : 2; }                 // as many as are resident
+int ln_fwd_blocks(int rows, int cols) { return std::min(ceil_div(rows, ln_rows_per_wg(cols)), ln_wgs_per_cu(cols) * kCUs); }
 int ln_bwd_blocks(int rows, int cols) {
-  return std::min(ceil_div(rows, ln_rows_per_wg(cols)), cols > 8192 ? kCUs : cols > 2048 ? 2 * kCUs : 4 * kCUs);
+  return std::min(ceil_div(rows, ln_rows_per_wg(cols)), (cols <= 2048 ? 4 : cols <= 8192 ? 2 : 1) * kCUs);
 }
 
 // ---- product: which kernel, and how many pieces the K axis is cut into
@@ -136,11 +137,11 @@ int snipper_fp8_quantize(void *stream, const void *x, int x_dtype, long long ldx
       using T = decltype(t);
       constexpr int F = decltype(f)::value;
       if (tile_rows == 128) {
-        if (mean) hipLaunchKernelGGL((quant_tile_kernel<T, F, true, true>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((quant_tile_kernel<T, F, true, false>), grid, dim3(256), 0, st, a);
+        if (mean) hipLaunchKernelGGL((quant_tile_kernel<T, F, true, true>), grid, dim3(512), 0, st, a);
+        else hipLaunchKernelGGL((quant_tile_kernel<T, F, true, false>), grid, dim3(512), 0, st, a);
       } else {
-        if (mean) hipLaunchKernelGGL((quant_tile_kernel<T, F, false, true>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((quant_tile_kernel<T, F, false, false>), grid, dim3(256), 0, st, a);
+        if (mean) hipLaunchKernelGGL((quant_tile_kernel<T, F, false, true>), grid, dim3(512), 0, st, a);
+        else hipLaunchKernelGGL((quant_tile_kernel<T, F, false, false>), grid, dim3(512), 0, st, a);
       }
     });
   });

@@ -52,61 +52,57 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs a) {
   }
 }
 
-// ---- both forms from one read.  A workgroup of four waves holds a 128 x 128 tile in registers: lane (i, l) = (lane >> 4, lane & 15)
-// of wave w the columns 8 l .. 8 l + 7 of rows 32 w + 16 h + 4 i + k (h < 2, k < 4).  Four consecutive rows in one lane make a 32-bit
+// ---- both forms from one read.  A workgroup of eight waves holds a 128 x 128 tile in registers: lane (i, l) = (lane >> 4, lane & 15)
+// of wave w the columns 8 l .. 8 l + 7 of rows 16 w + 4 i + k (k < 4); with four waves and twice the rows a lane the kernel took 192
+// registers and ran at two waves a SIMD.  Four consecutive rows in one lane make a 32-bit
 // word of the transposed form, which crosses LDS once (16-byte pieces XORed by the column's octet: reads are free of bank conflicts,
 // writes two-way) and is written as whole 128-byte lines.
 template <typename T, int FMT, bool TILE, bool NORM>
-__global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs a) {
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void quant_tile_kernel(QuantArgs a) {
   __shared__ __attribute__((aligned(16))) unsigned img[128 * 32];
-  __shared__ unsigned cmax[4][128];
-  __shared__ float csum[4][128];
+  __shared__ unsigned cmax[8][128];
+  __shared__ __attribute__((aligned(16))) unsigned cfin[128];
+  __shared__ float csum[8][128];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, i4 = lane >> 4;
   const int c0 = blockIdx.x * 128, c = c0 + 8 * l;
   const int rb = blockIdx.y + (int)blockIdx.z * 32768;
   const long long r0 = (long long)rb * 128;
   if (r0 >= a.R) return;                                   // (the whole workgroup)
-  float v[2][4][8];
+  float v[4][8];
   float gm[8], bt[8];
   if constexpr (NORM) {
     load_param8(a.gamma, a.p_dtype, c, a.C - c, 1.f, gm);
     load_param8(a.beta, a.p_dtype, c, a.C - c, 0.f, bt);
   }
   const int n = a.C - c;                                     // columns this lane has (8 of them unless the matrix ends)
-  const long long rl = r0 + 32 * wave + 4 * i4;
-  auto row_of = [&](int h, int k) { return rl + 16 * h + k; };
+  const long long rl = r0 + 16 * wave + 4 * i4;
+  auto row_of = [&](int k) { return rl + k; };
   if (n >= 8) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const long long r = row_of(h, k) < a.R ? row_of(h, k) : a.R - 1;
-        load8((const T *)a.x + r * a.ldx + c, 8, v[h][k]);
-      }
+    for (int k = 0; k < 4; ++k) {
+      const long long r = row_of(k) < a.R ? row_of(k) : a.R - 1;
+      load8((const T *)a.x + r * a.ldx + c, 8, v[k]);
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const long long r = row_of(h, k) < a.R ? row_of(h, k) : a.R - 1;
-          v[h][k][j] = j < n ? (float)((const T *)a.x)[r * a.ldx + c + j] : 0.f;
-        }
+      for (int k = 0; k < 4; ++k) {
+        const long long r = row_of(k) < a.R ? row_of(k) : a.R - 1;
+        v[k][j] = j < n ? (float)((const T *)a.x)[r * a.ldx + c + j] : 0.f;
+      }
   }
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+  for (int k = 0; k < 4; ++k) {
+    const bool in = row_of(k) < a.R;
+    if constexpr (NORM) {
+      const float mu = in ? a.mean[row_of(k)] : 0.f, rs = in ? a.rstd[row_of(k)] : 0.f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const bool in = row_of(h, k) < a.R;
-      if constexpr (NORM) {
-        const float mu = in ? a.mean[row_of(h, k)] : 0.f, rs = in ? a.rstd[row_of(h, k)] : 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[h][k][j] = j < n ? (v[h][k][j] - mu) * rs * gm[j] + bt[j] : 0.f;
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[h][k][j] = in ? v[h][k][j] : 0.f;
+      for (int j = 0; j < 8; ++j) v[k][j] = j < n ? (v[k][j] - mu) * rs * gm[j] + bt[j] : 0.f;
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[k][j] = in ? v[k][j] : 0.f;
+  }
   const long long P = pitch_of(a.C), Q = scales_of(a.C), Pt = pitch_of(a.R), Qt = scales_of(a.R);
   const int kb = blockIdx.x, last_kb = (int)((P >> 7) - 1), last_rb = (int)((Pt >> 7) - 1);
 
@@ -117,24 +113,34 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs a) {
     unsigned m = 0;
     float s = 0.f;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) { m = max(m, mag(v[h][k][j])); s += v[h][k][j]; }
+    for (int k = 0; k < 4; ++k) { m = max(m, mag(v[k][j])); s += v[k][j]; }
 #pragma unroll
     for (int o = 16; o <= 32; o <<= 1) {
       m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
       if (a.part) s += __shfl_xor(s, o, 64);
     }
-    cm[j] = m;
     if (i4 == 0) { cmax[wave][8 * l + j] = m; if (a.part) csum[wave][8 * l + j] = s; }
   }
   __syncthreads();
-  if (a.part && threadIdx.x < 128 && c0 + (int)threadIdx.x < a.C) {
+  if (threadIdx.x < 128) {
     const int t = threadIdx.x;
-    a.part[(long long)rb * a.C + c0 + t] = (csum[0][t] + csum[1][t]) + (csum[2][t] + csum[3][t]);
-  }
+    unsigned m = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) cm[j] = max(max(cmax[0][8 * l + j], cmax[1][8 * l + j]), max(cmax[2][8 * l + j], cmax[3][8 * l + j]));
+    for (int w = 0; w < 8; ++w) m = max(m, cmax[w][t]);
+    cfin[t] = m;
+    if (a.part && c0 + t < a.C) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) s += csum[w][t];
+      a.part[(long long)rb * a.C + c0 + t] = s;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 8; j += 4) {
+    const u32x4 m = *(const u32x4 *)(cfin + 8 * l + j);
+    cm[j] = m[0]; cm[j + 1] = m[1]; cm[j + 2] = m[2]; cm[j + 3] = m[3];
+  }
   unsigned all = 0;
   if constexpr (TILE) {
 #pragma unroll
@@ -145,26 +151,24 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs a) {
   // rows
   if (a.data) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int k = 0; k < 4; ++k) {
+      unsigned m = all;
+      if constexpr (!TILE) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        unsigned m = all;
-        if constexpr (!TILE) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) m = max(m, mag(v[h][k][j]));
-          m = max16(m);
-        }
-        const int byte = scale_byte<FMT>(m);
-        const float f = inv_scale(byte);
-        const float (&x)[8] = v[h][k];
-        const long long r = row_of(h, k);
-        if (r < a.R) {
-          const u32x2 w = {pack4<FMT>(x[0] * f, x[1] * f, x[2] * f, x[3] * f), pack4<FMT>(x[4] * f, x[5] * f, x[6] * f, x[7] * f)};
-          *(u32x2 *)(a.data + r * P + c) = w;
-          if (l == 0) a.scale[r * Q + kb] = (uint8_t)byte;
-          if (kb == last_kb && l > 0 && kb + l < Q) a.scale[r * Q + kb + l] = 127;
-        }
+        for (int j = 0; j < 8; ++j) m = max(m, mag(v[k][j]));
+        m = max16(m);
       }
+      const int byte = scale_byte<FMT>(m);
+      const float f = inv_scale(byte);
+      const float (&x)[8] = v[k];
+      const long long r = row_of(k);
+      if (r < a.R) {
+        const u32x2 w = {pack4<FMT>(x[0] * f, x[1] * f, x[2] * f, x[3] * f), pack4<FMT>(x[4] * f, x[5] * f, x[6] * f, x[7] * f)};
+        *(u32x2 *)(a.data + r * P + c) = w;
+        if (l == 0) a.scale[r * Q + kb] = (uint8_t)byte;
+        if (kb == last_kb && l > 0 && kb + l < Q) a.scale[r * Q + kb + l] = 127;
+      }
+    }
   }
   if (!a.data_t) return;
   // columns
@@ -173,11 +177,8 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs a) {
     const int byte = scale_byte<FMT>(TILE ? all : cm[j]);
     const float f = inv_scale(byte);
     const int cl = 8 * l + j;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int piece = (2 * wave + h) ^ (l & 7);                 // 16-byte piece of the column's line; (cl >> 3) & 7 = l & 7
-      img[cl * 32 + piece * 4 + i4] = pack4<FMT>(v[h][0][j] * f, v[h][1][j] * f, v[h][2][j] * f, v[h][3][j] * f);
-    }
+    const int piece = wave ^ (l & 7);                             // 16-byte piece of the column's line; (cl >> 3) & 7 = l & 7
+    img[cl * 32 + piece * 4 + i4] = pack4<FMT>(v[0][j] * f, v[1][j] * f, v[2][j] * f, v[3][j] * f);
     if (wave == 0 && i4 == 0 && c + j < a.C) {
       uint8_t *s = a.scale_t + (long long)(c + j) * Qt;
       s[rb] = (uint8_t)byte;
@@ -187,8 +188,8 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs a) {
   }
   __syncthreads();
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int idx = threadIdx.x + 256 * q, cl = idx >> 3, piece = idx & 7;
+  for (int q = 0; q < 2; ++q) {
+    const int idx = threadIdx.x + 512 * q, cl = idx >> 3, piece = idx & 7;
     if (c0 + cl < a.C)
       *(u32x4 *)(a.data_t + (long long)(c0 + cl) * Pt + r0 + piece * 16) = *(const u32x4 *)(img + cl * 32 + (piece ^ ((cl >> 3) & 7)) * 4);
   }

@@ -15,46 +15,72 @@ constexpr int kBlock = 128;                       // elements behind one scale
 
 enum { kF32 = 0, kBF16 = 1, kF16 = 3 };           // type codes of the C ABI
 
-// Eight consecutive elements of a row as float.  The address needs no more than the element's own alignment: memory instructions
-// take any on this hardware (a piece that straddles a cache line costs one more access), so odd widths and strides run the same
-// code as even ones.  `n` elements exist (n >= 8: all); the others read as 0.
-template <typename T>
-__device__ __forceinline__ void load8(const T *p, int n, float (&v)[8]) {
-  if (n >= 8) {
-    T t[8];
-    __builtin_memcpy(t, p, 8 * sizeof(T));
+// W consecutive elements of a row as float.  The address needs no more than the element's own alignment: memory instructions take any
+// on this hardware (a piece that straddles a cache line costs one more access), so odd widths and strides run the same code as even
+// ones.  `n` elements exist (n >= W: all); the others read as 0.
+template <int W, typename T>
+__device__ __forceinline__ void load_w(const T *p, int n, float (&v)[W]) {
+  if (n >= W) {
+    T t[W];
+    __builtin_memcpy(t, p, W * sizeof(T));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = (float)t[j];
+    for (int j = 0; j < W; ++j) v[j] = (float)t[j];
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < n ? (float)p[j] : 0.f;
+    for (int j = 0; j < W; ++j) v[j] = j < n ? (float)p[j] : 0.f;
   }
 }
-template <typename T>
-__device__ __forceinline__ void store8(T *p, int n, const float (&v)[8]) {
-  T t[8];
+template <int W, typename T>
+__device__ __forceinline__ void store_w(T *p, int n, const float (&v)[W]) {
+  T t[W];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) t[j] = (T)v[j];     // to nearest, ties to even
-  if (n >= 8) {
-    __builtin_memcpy(p, t, 8 * sizeof(T));
+  for (int j = 0; j < W; ++j) t[j] = (T)v[j];     // to nearest, ties to even
+  if (n >= W) {
+    __builtin_memcpy(p, t, W * sizeof(T));
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < W; ++j)
       if (j < n) p[j] = t[j];
   }
 }
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, int n, float (&v)[8]) { load_w<8>(p, n, v); }
+template <typename T>
+__device__ __forceinline__ void store8(T *p, int n, const float (&v)[8]) { store_w<8>(p, n, v); }
+// load_w in two halves, so that a loop can have the next row's elements on the way: what it reads, in the element's own type
+template <typename T, int W>
+struct Raw {
+  typedef T V __attribute__((ext_vector_type(W)));
+  V v;
+  __device__ __forceinline__ void load(const T *p, int n) {
+    if (n >= W) {
+      __builtin_memcpy(&v, p, W * sizeof(T));
+    } else {
+#pragma unroll
+      for (int j = 0; j < W; ++j) v[j] = j < n ? p[j] : (T)0.f;
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[W]) const {
+#pragma unroll
+    for (int j = 0; j < W; ++j) f[j] = (float)v[j];
+  }
+};
 // the same for parameters, whose type is known at run time only; a null pointer reads as `none`
-__device__ __forceinline__ void load_param8(const void *p, int dtype, long long at, int n, float none, float (&v)[8]) {
+template <int W>
+__device__ __forceinline__ void load_param_w(const void *p, int dtype, long long at, int n, float none, float (&v)[W]) {
   if (!p) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = none;
+    for (int j = 0; j < W; ++j) v[j] = none;
   } else if (dtype == kF32) {
-    load8((const float *)p + at, n, v);
+    load_w<W>((const float *)p + at, n, v);
   } else if (dtype == kBF16) {
-    load8((const bf16_t *)p + at, n, v);
+    load_w<W>((const bf16_t *)p + at, n, v);
   } else {
-    load8((const f16_t *)p + at, n, v);
+    load_w<W>((const f16_t *)p + at, n, v);
   }
+}
+__device__ __forceinline__ void load_param8(const void *p, int dtype, long long at, int n, float none, float (&v)[8]) {
+  load_param_w<8>(p, dtype, at, n, none, v);
 }
 __device__ __forceinline__ float load_param(const void *p, int dtype, long long at) {
   return dtype == kF32 ? ((const float *)p)[at] : dtype == kBF16 ? (float)((const bf16_t *)p)[at] : (float)((const f16_t *)p)[at];
@@ -96,14 +122,16 @@ __device__ __forceinline__ unsigned pack4(float a, float b, float c, float d) {
   return (unsigned)r;
 }
 
-__device__ __forceinline__ unsigned max16(unsigned v) {        // over the 16 lanes of a row of the wave
+template <int L>
+__device__ __forceinline__ unsigned max_over(unsigned v) {     // over L neighbouring lanes
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
+  for (int o = L / 2; o > 0; o >>= 1) {
     const unsigned t = (unsigned)__shfl_xor((int)v, o, 64);
     v = v > t ? v : t;
   }
   return v;
 }
+__device__ __forceinline__ unsigned max16(unsigned v) { return max_over<16>(v); }
 
 }  // namespace rows
 }  // namespace snipper
