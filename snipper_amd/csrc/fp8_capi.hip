@@ -145,7 +145,7 @@ int snipper_fp8_quantize(void *stream, const void *x, int x_dtype, long long ldx
       }
     });
   });
-  if (colsum) hipLaunchKernelGGL(colsum_parts_kernel, dim3(ceil_div(cols, 8)), dim3(256), 0, st, (const float *)workspace, rb, cols, colsum);
+  if (colsum) hipLaunchKernelGGL(colsum_parts_kernel, dim3(ceil_div(cols, 32)), dim3(1024), 0, st, (const float *)workspace, rb, cols, colsum);
   return launch_status();
 }
 
@@ -180,12 +180,12 @@ int snipper_fp8_matmul(void *stream, const uint8_t *A, const uint8_t *a_scale, i
           else if (p.row_tiles == 2) hipLaunchKernelGGL((mm_rows_kernel<FA, FB, E, 2>), grid, block, lds, st, a);
           else hipLaunchKernelGGL((mm_rows_kernel<FA, FB, E, 4>), grid, block, lds, st, a);
         } else if (p.kind == 1) {
-          hipLaunchKernelGGL((mm_tile_kernel<FA, FB, E, 2, 2, 4, 4, false>), dim3(p.tiles, p.splits), dim3(256), 0, st, a);
+          hipLaunchKernelGGL((mm_tile_kernel<FA, FB, E, 2, 2, 4, 4, false>), dim3(p.tiles * p.splits), dim3(256), 0, st, a);
         } else if constexpr (E) {
         } else if (p.kind == 3) {
           launch_stationary<FA, FB>(a, p.tiles, st);
         } else {
-          hipLaunchKernelGGL((mm_tile_kernel<FA, FB, false, 2, 4, 8, 4, true>), dim3(p.tiles, p.splits), dim3(512), 0, st, a);
+          hipLaunchKernelGGL((mm_tile_kernel<FA, FB, false, 2, 4, 8, 4, true>), dim3(p.tiles * p.splits), dim3(512), 0, st, a);
         }
       };
       if (exact) go(std::true_type{});
@@ -248,7 +248,7 @@ int snipper_layernorm_backward(void *stream, const void *g, const void *x, int x
       });
     });
   if (dgamma)
-    hipLaunchKernelGGL(ln_rows_join_kernel, dim3(ceil_div(2 * cols, 8)), dim3(256), 0, st, (const float *)workspace, blocks, cols, dgamma, dbeta, p_dtype);
+    hipLaunchKernelGGL(ln_rows_join_kernel, dim3(ceil_div(2 * cols, 32)), dim3(1024), 0, st, (const float *)workspace, blocks, cols, dgamma, dbeta, p_dtype);
   return launch_status();
 }
 

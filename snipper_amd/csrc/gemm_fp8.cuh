@@ -165,16 +165,18 @@ __global__ __launch_bounds__(64 * WM * WN) void mm_tile_kernel(MmArgs a) {
   const int wm = wave / WN, wn = wave - wm * WN;
   const int r = lane & 15, g = lane >> 4;
 
-  // workgroup -> tile: each XCD (ids modulo 8) walks a contiguous run of tiles, column tiles of eight row tiles at a time
+  // workgroup -> piece of the K axis and tile: each XCD (ids modulo 8) walks a contiguous run, so that the tiles of a piece, which share
+  // its rows' bytes, are on one XCD; within a piece column tiles of eight row tiles at a time
   const int tm_n = (a.M + BM - 1) / BM, tn_n = (a.N + BN - 1) / BN, tiles = tm_n * tn_n;
-  const int id = blockIdx.x, per = tiles >> 3, rem = tiles & 7, xcd = id & 7;
-  const int t = xcd * per + (xcd < rem ? xcd : rem) + (id >> 3);
+  const int id = blockIdx.x, all = tiles * a.splits, per = all >> 3, rem = all & 7, xcd = id & 7;
+  const int at = xcd * per + (xcd < rem ? xcd : rem) + (id >> 3);
+  const int split = at / tiles, t = at - split * tiles;
   const int band = t / (8 * tn_n), in_band = t - band * 8 * tn_n, bh = min(8, tm_n - band * 8);
   int m0 = (band * 8 + in_band % bh) * BM, n0 = (in_band / bh) * BN;
   if constexpr (INWARD) { m0 = min(m0, a.M - BM); n0 = min(n0, a.N - BN); }
 
   const long long P = (long long)a.steps * 128, Q = (long long)((a.steps + 3) >> 2) * 4;
-  const int k_begin = blockIdx.y * a.per_split, k_end = min(a.steps, k_begin + a.per_split);
+  const int k_begin = split * a.per_split, k_end = min(a.steps, k_begin + a.per_split);
 
   const int rows_a = min(BM, a.M - m0), rows_b = min(BN, a.N - n0);
   static_assert((BM / 8) % kWaves == 0 && kWaves % 2 == 0, "an instruction's side is known at compile time, its parity the wave's");
@@ -269,7 +271,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mm_tile_kernel(MmArgs a) {
       float v[8];
 #pragma unroll
       for (int q = 0; q < 4; ++q) { v[q] = acc[i][j][q]; v[4 + q] = acc[i][j + 1][q]; }
-      if (a.part) store8(a.part + ((long long)blockIdx.y * a.M + m) * a.N + n, a.N - n, v);
+      if (a.part) store8(a.part + ((long long)split * a.M + m) * a.N + n, a.N - n, v);
       else mm_store(a, m, n, v, bias);
     }
   }

@@ -85,11 +85,13 @@ __global__ __launch_bounds__(ln_threads(LPR)) void ln_rows_fwd_kernel(LnRowsArgs
       raw[p].load((const T *)a.x + (in ? row * a.ldx + c : 0), in ? a.C - c : 0);
     }
   };
-  fetch((long long)blockIdx.x * RPW + sub);
+  constexpr bool AHEAD = NIT == 1;                      // (with more the registers cost more waves than the early loads gain)
+  if (AHEAD) fetch((long long)blockIdx.x * RPW + sub);
   // every thread of a workgroup makes the same number of rounds (there are barriers inside where LPR > 64)
   for (long long r0 = (long long)blockIdx.x * RPW; r0 < a.R; r0 += (long long)gridDim.x * RPW) {
     const long long row = r0 + sub;
     const bool in = row < a.R;
+    if (!AHEAD) fetch(row);
     float v[NP][W];
     float s[1] = {0.f};
 #pragma unroll
@@ -98,7 +100,7 @@ __global__ __launch_bounds__(ln_threads(LPR)) void ln_rows_fwd_kernel(LnRowsArgs
 #pragma unroll
       for (int j = 0; j < W; j += 4) s[0] += (v[p][j] + v[p][j + 1]) + (v[p][j + 2] + v[p][j + 3]);
     }
-    fetch(row + (long long)gridDim.x * RPW);            // the next row, while this one is worked on
+    if (AHEAD) fetch(row + (long long)gridDim.x * RPW); // the next row, while this one is worked on
     ln_row_sums<LPR, 1>(s, red, 0);
     const float mean = s[0] * inv;
     float q[1] = {0.f};
@@ -171,7 +173,7 @@ __global__ __launch_bounds__(ln_threads(LPR)) void ln_rows_bwd_kernel(LnRowsArgs
       rg[p].load((const T *)a.g + (in ? row * a.C + c : 0), n);
     }
   };
-  constexpr bool AHEAD = LPR * NIT < 2048;              // (1024 threads have 128 registers each: the widest rows are fetched in turn)
+  constexpr bool AHEAD = NIT == 1;
   if (AHEAD) fetch((long long)blockIdx.x * RPW + sub);
   int turn = 0;
   for (long long r0 = (long long)blockIdx.x * RPW; r0 < a.R; r0 += (long long)gridDim.x * RPW, turn ^= 1) {
@@ -243,23 +245,11 @@ __global__ __launch_bounds__(ln_threads(LPR)) void ln_rows_bwd_kernel(LnRowsArgs
   }
 }
 
-// dgamma[c] = sum_b part[b][0][c], dbeta[c] = sum_b part[b][1][c]: 8 columns x 32 slices of b per workgroup, a fixed order
-__global__ __launch_bounds__(256) void ln_rows_join_kernel(const float *part, int nparts, int C, void *dgamma, void *dbeta, int p_dtype) {
-  __shared__ float red[32][9];
-  const int ci = threadIdx.x & 7, slice = threadIdx.x >> 3, e = blockIdx.x * 8 + ci;           // over 2 C
-  float s = 0.f;
-  if (e < 2 * C) {
-#pragma unroll 8
-    for (int b = slice; b < nparts; b += 32) s += part[(long long)b * 2 * C + e];
-  }
-  red[slice][ci] = s;
-  __syncthreads();
-  if (slice == 0 && e < 2 * C) {
-    s = 0.f;
-#pragma unroll
-    for (int k = 0; k < 32; ++k) s += red[k][ci];
-    store_param(e < C ? dgamma : dbeta, p_dtype, e < C ? e : e - C, s);
-  }
+// dgamma[c] = sum_b part[b][0][c], dbeta[c] = sum_b part[b][1][c]
+__global__ __launch_bounds__(1024) void ln_rows_join_kernel(const float *part, int nparts, int C, void *dgamma, void *dbeta, int p_dtype) {
+  const int e = blockIdx.x * 32 + (threadIdx.x & 31);          // over 2 C
+  const float s = sum_parts(part, nparts, 2 * C, e);
+  if (threadIdx.x < 32 && e < 2 * C) store_param(e < C ? dgamma : dbeta, p_dtype, e < C ? e : e - C, s);
 }
 
 }  // namespace rows

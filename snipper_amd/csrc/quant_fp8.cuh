@@ -58,7 +58,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs a) {
 // word of the transposed form, which crosses LDS once (16-byte pieces XORed by the column's octet: reads are free of bank conflicts,
 // writes two-way) and is written as whole 128-byte lines.
 template <typename T, int FMT, bool TILE, bool NORM>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void quant_tile_kernel(QuantArgs a) {
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(NORM ? 5 : 6))) void quant_tile_kernel(QuantArgs a) {
   __shared__ __attribute__((aligned(16))) unsigned img[128 * 32];
   __shared__ unsigned cmax[8][128];
   __shared__ __attribute__((aligned(16))) unsigned cfin[128];
@@ -183,7 +183,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void q
       uint8_t *s = a.scale_t + (long long)(c + j) * Qt;
       s[rb] = (uint8_t)byte;
       if (rb == last_rb)
-        for (long long t = rb + 1; t < Qt; ++t) s[t] = 127;
+        for (int t = rb + 1; t < Qt; ++t) s[t] = 127;
     }
   }
   __syncthreads();
@@ -195,23 +195,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void q
   }
 }
 
-// out[c] = sum_b part[b][c]: 8 columns x 32 slices of b per workgroup, a fixed order
-__global__ __launch_bounds__(256) void colsum_parts_kernel(const float *part, int nparts, int C, float *out) {
-  __shared__ float red[32][9];
-  const int ci = threadIdx.x & 7, slice = threadIdx.x >> 3, c = blockIdx.x * 8 + ci;
-  float s = 0.f;
-  if (c < C) {
-#pragma unroll 8
-    for (int b = slice; b < nparts; b += 32) s += part[(long long)b * C + c];
-  }
-  red[slice][ci] = s;
-  __syncthreads();
-  if (slice == 0 && c < C) {
-    s = 0.f;
-#pragma unroll
-    for (int k = 0; k < 32; ++k) s += red[k][ci];
-    out[c] = s;
-  }
+// out[c] = sum_b part[b][c]
+__global__ __launch_bounds__(1024) void colsum_parts_kernel(const float *part, int nparts, int C, float *out) {
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31);
+  const float s = sum_parts(part, nparts, C, c);
+  if (threadIdx.x < 32 && c < C) out[c] = s;
 }
 
 }  // namespace rows

@@ -91,6 +91,26 @@ __device__ __forceinline__ void store_param(void *p, int dtype, long long at, fl
   else ((f16_t *)p)[at] = (f16_t)v;
 }
 
+// sum_b part[b][e] of nparts rows of `width`, for threads 0 .. 31 of a workgroup of 1024, each an element e: 32 elements (a line of 128
+// bytes) x 32 slices of b that meet in LDS, in a fixed order
+__device__ __forceinline__ float sum_parts(const float *part, int nparts, int width, int e) {
+  __shared__ float red[32][33];
+  const int i = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  float s = 0.f;
+  if (e < width) {
+#pragma unroll 8
+    for (int b = slice; b < nparts; b += 32) s += part[(long long)b * width + e];
+  }
+  red[slice][i] = s;
+  __syncthreads();
+  s = 0.f;
+  if (slice == 0) {
+#pragma unroll
+    for (int k = 0; k < 32; ++k) s += red[k][i];
+  }
+  return s;
+}
+
 // ---- the scale of a block -------------------------------------------------------------------------------------------
 // Magnitude that counts for the scale: |x| of a finite x, 0 of an infinity or NaN.  As bits, so that a maximum is one of integers.
 __device__ __forceinline__ unsigned mag(float x) {
