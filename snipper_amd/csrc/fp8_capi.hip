@@ -60,35 +60,41 @@ int ln_bwd_blocks(int rows, int cols) {
   return std::min(ceil_div(rows, ln_rows_per_wg(cols)), (cols <= 2048 ? 4 : cols <= 8192 ? 2 : 1) * kCUs);
 }
 
-// ---- product: which kernel, and how many pieces the K axis is cut into
+// ---- product: which kernel, and how many pieces the K axis is cut into (times in us of bfloat16 results, M x N x K, 256 CUs)
 struct MmPlan {
-  int kind;                  // 0 few rows, 1 tiles of 128 x 128, 2 tiles of 256 x 256, 3 B in registers
-  int tiles, splits, per_split, waves, row_tiles;
+  int kind;                  // 0 few rows, 1 tiles of 128 x 128, 2 tiles of 256 x 256, 3 B in registers, 4 tiles of 64 x 64
+  int tiles, splits, per_split, waves;
 };
 MmPlan mm_plan(int M, int N, int K, bool exact) {
   MmPlan p{};
   const int steps = ceil_div(K, 128);
   p.splits = 1;
   p.per_split = steps;
-  if (M <= 64) {
-    p.row_tiles = M <= 16 ? 1 : M <= 32 ? 2 : 4;
-    p.waves = std::max(1, std::min(16, steps / 4));
+  // one operand of rows: 16 x 4096 x 4096 7.8 against 8.3 in tiles; 33 rows 12.1 (a second and third pass over A's operands) against 9.4
+  if (M <= 16) {
+    p.waves = std::max(1, std::min(8, ceil_div(steps, 4)));
     return p;
   }
-  // K <= 1024: loads and stores bound such products, and the kernel with B in registers overlaps them; whole 16-byte pieces of rows
-  // only, and at least as many chunks of 64 rows as there are CUs
+  // K <= 1024: loads and stores bound such products, and the kernel with B in registers overlaps them.  Whole 16-byte pieces of rows
+  // only, and at least as many chunks of 64 rows as there are CUs.  79 000 x 1024 x 384 52 against 100, 16 384 x 1024 x 1024 27 against
+  // 28, 4096 x 4096 x 512 18 against 21; with fewer chunks 1024^3 13 against 6
   if (!exact && steps <= 8 && N % 8 == 0 && (long long)ceil_div(M, 64) * ceil_div(N, 256) >= kCUs && (long long)N * 128 <= 0x7fffffff) {
     p.kind = 3;
     p.tiles = std::max(1, kCUs / (8 * ceil_div(N, 256))) * 8;     // chunk lists: one workgroup per CU
     return p;
   }
-  const long long big = (long long)ceil_div(M, 256) * ceil_div(N, 256);
-  p.kind = !exact && M >= 256 && N >= 256 && big >= kCUs ? 2 : 1;
-  const int edge = p.kind == 2 ? 256 : 128;
+  // The largest tile that still gives every CU one: 4096^3 66 (256) against 71 (128); 8192 x 1024 x 4096 38 (128) against 57 (256), 55
+  // (64); 1024^3 6 (64) against 10 (128).  Few tiles and a long K axis: larger tiles, which load less, and more pieces
+  const long long t128 = (long long)ceil_div(M, 128) * ceil_div(N, 128);
+  if (!exact && M >= 256 && N >= 256 && (long long)ceil_div(M, 256) * ceil_div(N, 256) >= kCUs) p.kind = 2;
+  else p.kind = t128 >= kCUs || steps >= 64 ? 1 : 4;
+  const int edge = p.kind == 2 ? 256 : p.kind == 1 ? 128 : 64;
   p.tiles = ceil_div(M, edge) * ceil_div(N, edge);
-  if (p.tiles < 2 * kCUs && steps >= 8) {
-    const int want = std::min(ceil_div(2 * kCUs, p.tiles), steps / 4);
-    p.per_split = ceil_div(ceil_div(steps, std::max(1, want)), 4) * 4;
+  // pieces of at least 8 steps, up to one workgroup of 64 x 64 or two of 128 x 128 per CU: 33 x 4096 x 4096 11 -> 9.4, 100 x 4096 x
+  // 4096 11.5 -> 10.7; 256 x 4096 x 4096, a tile per CU, 12.2 -> 15.8, and cut at 128 x 128 8192 x 1024 x 4096 38 -> 61
+  const int want = std::min((p.kind == 1 && t128 < kCUs ? 2 : 1) * kCUs / p.tiles, steps / 8);
+  if (p.kind != 2 && want > 1) {
+    p.per_split = ceil_div(ceil_div(steps, want), 4) * 4;
     p.splits = ceil_div(steps, p.per_split);
   }
   return p;
@@ -174,11 +180,9 @@ int snipper_fp8_matmul(void *stream, const uint8_t *A, const uint8_t *a_scale, i
       auto go = [&](auto ex) {
         constexpr bool E = decltype(ex)::value;
         if (p.kind == 0) {
-          const dim3 grid(ceil_div(N, 16), ceil_div(M, 16 * p.row_tiles)), block(64 * p.waves);
-          const size_t lds = (size_t)p.waves * p.row_tiles * 64 * 16;
-          if (p.row_tiles == 1) hipLaunchKernelGGL((mm_rows_kernel<FA, FB, E, 1>), grid, block, lds, st, a);
-          else if (p.row_tiles == 2) hipLaunchKernelGGL((mm_rows_kernel<FA, FB, E, 2>), grid, block, lds, st, a);
-          else hipLaunchKernelGGL((mm_rows_kernel<FA, FB, E, 4>), grid, block, lds, st, a);
+          hipLaunchKernelGGL((mm_rows_kernel<FA, FB, E>), dim3(ceil_div(N, 16)), dim3(64 * p.waves), 0, st, a);
+        } else if (p.kind == 4) {
+          hipLaunchKernelGGL((mm_tile_kernel<FA, FB, E, 2, 2, 2, 2, false>), dim3(p.tiles * p.splits), dim3(256), 0, st, a);
         } else if (p.kind == 1) {
           hipLaunchKernelGGL((mm_tile_kernel<FA, FB, E, 2, 2, 4, 4, false>), dim3(p.tiles * p.splits), dim3(256), 0, st, a);
         } else if constexpr (E) {

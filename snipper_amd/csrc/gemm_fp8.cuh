@@ -144,6 +144,10 @@ __device__ __forceinline__ void dma4(const uint8_t *base, int range, unsigned ch
 template <int N>
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
+// f(0), f(1), ... with constants
+template <typename F, int... K>
+__device__ __forceinline__ void each_step(F &&f, std::integer_sequence<int, K...>) { (f(std::integral_constant<int, K>{}), ...); }
+
 // ---- tiles -----------------------------------------------------------------------------------------------------------
 // A workgroup of WM x WN waves makes a (16 TM WM) x (16 TN WN) tile; a K step of 128 is one byte-row of 128 per row of either side.
 // Rows go to LDS by DMA in 16-byte pieces, piece c of row r at place c ^ key(r), and a lane takes pieces g and g + 4 of its row (both
@@ -299,10 +303,6 @@ __global__ __launch_bounds__(256) void mm_join_kernel(MmArgs a) {
   }
 }
 
-// f(0), f(1), ... with constants
-template <typename F, int... K>
-__device__ __forceinline__ void each_step(F &&f, std::integer_sequence<int, K...>) { (f(std::integral_constant<int, K>{}), ...); }
-
 // the loads of a chunk of 64 rows and of its scale words, KS + ceil(KS / 4) instructions of every wave; behind the last chunk the range
 // is empty: zeros for a slot that nobody reads
 template <int KS>
@@ -421,51 +421,50 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 }
 
 // ---- few rows -----------------------------------------------------------------------------------------------------------
-// At most 16 T rows of A: B's bytes count, and they are read once, straight into registers.  A workgroup of W waves makes 16 columns;
-// the waves take every W-th K step and add their sums through LDS in a fixed order.
-template <int FA, int FB, bool EXACT, int T>
-__global__ __launch_bounds__(1024) void mm_rows_kernel(MmArgs a) {
-  extern __shared__ f32x4 red[];                                // [W][T][64]
+// At most 16 rows of A: B's bytes count, and they are read once, straight into registers.  A workgroup of W waves makes 16 columns; the
+// waves take every W-th group of four K steps (a word of scales; all of a group's loads are on the way before its first product) and
+// add their sums through LDS in a fixed order.
+template <int FA, int FB, bool EXACT>
+__global__ __launch_bounds__(512) void mm_rows_kernel(MmArgs a) {
+  __shared__ f32x4 red[8][64];
   const int lane = threadIdx.x & 63, W = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * T;
+  const int n0 = blockIdx.x * 16;
   const long long P = (long long)a.steps * 128, Q = (long long)((a.steps + 3) >> 2) * 4;
-  const long long nb = min(n0 + r, a.N - 1);
-  const uint8_t *bp = a.B + nb * P + g * 32, *sbp = a.sB + nb * Q;
-  const uint8_t *ap[T], *sap[T];
-  f32x4 acc[T];
+  const long long nb = min(n0 + r, a.N - 1), m = min(r, a.M - 1);
+  const uint8_t *bp = a.B + nb * P + g * 32, *sbp = a.sB + nb * Q, *ap = a.A + m * P + g * 32, *sap = a.sA + m * Q;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int kg = wave; kg < (a.steps + 3) >> 2; kg += W) {
+    const int sb = *(const int *)(sbp + kg * 4), sa = *(const int *)(sap + kg * 4);
+    i32x4 b[4][2], x[4][2];
 #pragma unroll
-  for (int i = 0; i < T; ++i) {
-    const long long m = min(m0 + 16 * i + r, a.M - 1);
-    ap[i] = a.A + m * P + g * 32;
-    sap[i] = a.sA + m * Q;
-    acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  for (int kt = wave; kt < a.steps; kt += W) {
-    const long long at = (long long)kt * 128;
-    Operand<FB, EXACT> b;
-    const int sb = sbp[kt];
-    b.set(*(const i32x4 *)(bp + at), *(const i32x4 *)(bp + at + 16), sb, 0);
-#pragma unroll
-    for (int i = 0; i < T; ++i) {
-      Operand<FA, EXACT> x;
-      const int sa = sap[i][kt];
-      x.set(*(const i32x4 *)(ap[i] + at), *(const i32x4 *)(ap[i] + at + 16), sa, 0);
-      acc[i] = mm_step<FB, FA, 0>(b, x, acc[i], sb, sa);
+    for (int q = 0; q < 4; ++q) {
+      const long long at = min(kg * 4 + q, a.steps - 1) * 128ll;        // (a step behind the last one: loaded, not used)
+      b[q][0] = *(const i32x4 *)(bp + at);
+      b[q][1] = *(const i32x4 *)(bp + at + 16);
+      x[q][0] = *(const i32x4 *)(ap + at);
+      x[q][1] = *(const i32x4 *)(ap + at + 16);
     }
+    each_step([&](auto step) {
+      constexpr int S = decltype(step)::value;
+      if (kg * 4 + S < a.steps) {
+        Operand<FB, EXACT> o;
+        Operand<FA, EXACT> i;
+        o.set(b[S][0], b[S][1], sb, S);
+        i.set(x[S][0], x[S][1], sa, S);
+        acc = mm_step<FB, FA, S>(o, i, acc, sb, sa);
+      }
+    }, std::make_integer_sequence<int, 4>{});
   }
-#pragma unroll
-  for (int i = 0; i < T; ++i) red[(wave * T + i) * 64 + lane] = acc[i];
+  red[wave][lane] = acc;
   __syncthreads();
-  for (int i = wave; i < T; i += W) {
-    f32x4 v = red[i * 64 + lane];
-    for (int w = 1; w < W; ++w) v += red[(w * T + i) * 64 + lane];
-    const long long m = m0 + 16 * i + r;
-    const float o[4] = {v[0], v[1], v[2], v[3]};
+  if (wave == 0) {
+    for (int w = 1; w < W; ++w) acc += red[w][lane];
+    const float o[4] = {acc[0], acc[1], acc[2], acc[3]};
     float bias[4];
     mm_bias(a, n0 + 4 * g, bias);
-    if (m < a.M) mm_store(a, m, n0 + 4 * g, o, bias);
+    if (r < a.M) mm_store(a, r, n0 + 4 * g, o, bias);
   }
 }
 
