@@ -21,11 +21,10 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._autograd import Function
-from .fused import _ROW_DT, _layer_norm_backward, _layer_norm_forward, _norm_rows, _opt
+from .fused import _ROW_DT, _call, _layer_norm_backward, _layer_norm_forward, _norm_rows, _once_differentiable, _opt
 
 _FMT = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}
 _MAX_DIM = 1 << 23
@@ -41,10 +40,10 @@ class Fp8Blocks:
     def __init__(self, data: torch.Tensor, scale: torch.Tensor, cols: int):
         if data.dtype not in _FMT or scale.dtype is not torch.float8_e8m0fnu:
             raise TypeError(f"Fp8Blocks: data in float8_e4m3fn or float8_e5m2 and scale in float8_e8m0fnu, got {data.dtype} and {scale.dtype}")
-        if (cols < 1 or data.dim() != 2 or data.shape[1] != -(-cols // 128) * 128 or
-                scale.shape != (data.shape[0], -(-cols // 512) * 4)):
-            raise ValueError(f"Fp8Blocks: data {tuple(data.shape)} and scale {tuple(scale.shape)} are not those of {cols} columns")
-        if not data.is_contiguous() or not scale.is_contiguous() or data.device != scale.device:
+        shape = data.shape
+        if cols < 1 or len(shape) != 2 or shape[1] != -(-cols // 128) * 128 or scale.shape != (shape[0], -(-cols // 512) * 4):
+            raise ValueError(f"Fp8Blocks: data {tuple(shape)} and scale {tuple(scale.shape)} are not those of {cols} columns")
+        if not (data.is_contiguous() and scale.is_contiguous()) or data.device != scale.device:
             raise ValueError("Fp8Blocks: data and scale are contiguous and on one device")
         self.data, self.scale, self.cols = data, scale, cols
 
@@ -59,9 +58,32 @@ class Fp8Blocks:
         return (self.data.float().view(R, P // 128, 128) * s[:, :, None]).view(R, P)[:, :self.cols]
 
 
-def _empty_blocks(rows: int, cols: int, dtype, device):
-    return (torch.empty((rows, -(-cols // 128) * 128), dtype=dtype, device=device),
-            torch.empty((rows, -(-cols // 512) * 4), dtype=torch.float8_e8m0fnu, device=device))
+class _Held:
+    """The same inside this file: pointers into one buffer (or into an Fp8Blocks' tensors), so that a training step makes few tensors."""
+
+    __slots__ = ("keep", "data", "scale", "rows", "cols", "fmt")
+
+    def __init__(self, keep, data, scale, rows, cols, fmt):
+        self.keep, self.data, self.scale, self.rows, self.cols, self.fmt = keep, data, scale, rows, cols, fmt
+
+    @staticmethod
+    def new(rows: int, cols: int, fmt: int, device) -> "_Held":
+        n = rows * (-(-cols // 128) * 128)
+        return _Held.of(torch.empty(n + rows * (-(-cols // 512) * 4), dtype=torch.uint8, device=device), rows, cols, fmt)
+
+    @staticmethod
+    def of(buf, rows: int, cols: int, fmt: int) -> "_Held":
+        p = buf.data_ptr()
+        return _Held(buf, p, p + rows * (-(-cols // 128) * 128), rows, cols, fmt)
+
+    @staticmethod
+    def view(b: Fp8Blocks) -> "_Held":
+        return _Held(b, b.data.data_ptr(), b.scale.data_ptr(), b.data.shape[0], b.cols, _FMT[b.data.dtype])
+
+
+def _new_blocks(rows: int, cols: int, dtype, device) -> Fp8Blocks:
+    return Fp8Blocks(torch.empty((rows, -(-cols // 128) * 128), dtype=dtype, device=device),
+                     torch.empty((rows, -(-cols // 512) * 4), dtype=torch.float8_e8m0fnu, device=device), cols)
 
 
 def _matrix(x: torch.Tensor, what: str):
@@ -70,15 +92,20 @@ def _matrix(x: torch.Tensor, what: str):
         raise RuntimeError(f"{what}: Not implemented on the CPU")
     if x.dtype not in _ROW_DT:
         raise TypeError(f"{what}: float32, bfloat16 or float16, got {x.dtype}")
-    if x.dim() < 2:
-        raise ValueError(f"{what}: a matrix or a batch of rows, got {tuple(x.shape)}")
-    C = x.shape[-1]
-    x2 = x if x.dim() == 2 else x.reshape(-1, C) if C else x
-    if not 1 <= C <= _MAX_DIM or x2.shape[0] > _MAX_DIM:
-        raise ValueError(f"{what}: up to 2^23 rows of 1 to 2^23 elements, got {tuple(x.shape)}")
-    if x2.stride(1) != 1 or (x2.shape[0] > 1 and x2.stride(0) < C):
-        x2 = x2.contiguous()
-    return x2, (x2.stride(0) if x2.shape[0] > 1 else C)
+    shape = x.shape
+    if len(shape) < 2:
+        raise ValueError(f"{what}: a matrix or a batch of rows, got {tuple(shape)}")
+    C = shape[-1]
+    x2 = x if len(shape) == 2 else x.reshape(-1, C) if C else x
+    R = x2.shape[0]
+    if not 1 <= C <= _MAX_DIM or R > _MAX_DIM:
+        raise ValueError(f"{what}: up to 2^23 rows of 1 to 2^23 elements, got {tuple(shape)}")
+    if R <= 1 and x2.stride(1) == 1:
+        return x2, C
+    ld, inner = x2.stride()
+    if inner != 1 or ld < C:
+        x2, ld = x2.contiguous(), C
+    return x2, ld
 
 
 def _format(dtype, what: str) -> int:
@@ -92,63 +119,65 @@ def _no_graph(what: str, *tensors) -> None:
         raise RuntimeError(f"{what} is not differentiable: use linear_fp8 / layer_norm_linear_fp8, or call it under torch.no_grad()")
 
 
-def _quantize(x2, ld, dtype, rows=True, cols=False, tile=False, colsum=False, norm=None):
-    """(blocks of x or None, blocks of x^T or None, column sums or None), as tensors.  ``norm``: (stats [2, R], gamma, beta, p_dtype)."""
-    fmt = _FMT[dtype]
+def _quantize(x2, ld, fmt, a=None, b=None, tile=False, colsum=False, norm=None):
+    """x into a (blocks of x) and / or b (blocks of x^T); the sums over the rows if ``colsum``.  ``norm``: (stats [2, R], gamma, beta,
+    p_dtype)."""
     R, C = x2.shape
     dev = x2.device
-    a = _empty_blocks(R, C, dtype, dev) if rows else None
-    b = _empty_blocks(C, R, dtype, dev) if cols else None
-    s = torch.empty(C, dtype=torch.float32, device=dev) if colsum else None
-    stats, gamma, beta, p_dtype = norm if norm is not None else (None, None, None, torch.float32)
     lib = _lib.load()
-    nbytes = lib.snipper_fp8_quantize_workspace_bytes(R, C, 1) if colsum else 0
-    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=dev) if nbytes else None
-    with _lib.device_guard(dev):
-        rc = lib.snipper_fp8_quantize(
-            _lib.raw_stream(dev), x2.data_ptr(), _ROW_DT[x2.dtype], ld, R, C, 128 if tile else 1, fmt,
-            stats[0].data_ptr() if norm is not None else None, stats[1].data_ptr() if norm is not None else None, _opt(gamma), _opt(beta),
-            _ROW_DT[p_dtype], a[0].data_ptr() if rows else None, a[1].data_ptr() if rows else None, b[0].data_ptr() if cols else None,
-            b[1].data_ptr() if cols else None, _opt(s), _opt(ws), nbytes)
-    _lib.check(rc, "snipper_fp8_quantize")
-    return a, b, s
+    s = ws = None
+    nbytes = 0
+    if colsum:
+        nbytes = lib.snipper_fp8_quantize_workspace_bytes(R, C, 1)
+        s, ws = torch.empty(C, dtype=torch.float32, device=dev), torch.empty(nbytes // 4, dtype=torch.float32, device=dev)
+    mean = rstd = gamma = beta = None
+    p_dtype = 0
+    if norm is not None:
+        mean, gamma, beta, p_dtype = norm[0].data_ptr(), _opt(norm[1]), _opt(norm[2]), _ROW_DT[norm[3]]
+        rstd = mean + 4 * R
+    _call(lib.snipper_fp8_quantize, dev, x2.data_ptr(), _ROW_DT[x2.dtype], ld, R, C, 128 if tile else 1, fmt, mean, rstd, gamma, beta, p_dtype,
+          a.data if a is not None else None, a.scale if a is not None else None, b.data if b is not None else None,
+          b.scale if b is not None else None, _opt(s), _opt(ws), nbytes)
+    return s
 
 
 def quantize_rows(x: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> Fp8Blocks:
     """x [..., cols] (float32 / bfloat16 / float16, leading axes as rows) into blocks of 128 elements of a row."""
-    _format(dtype, "quantize_rows")
+    fmt = _format(dtype, "quantize_rows")
     _no_graph("quantize_rows", x)
     x2, ld = _matrix(x, "quantize_rows")
-    if x2.shape[0] == 0:
-        return Fp8Blocks(*_empty_blocks(0, x2.shape[1], dtype, x.device), x2.shape[1])
-    return Fp8Blocks(*_quantize(x2, ld, dtype)[0], x2.shape[1])
+    a = _new_blocks(*x2.shape, dtype, x.device)
+    if x2.shape[0]:
+        _quantize(x2, ld, fmt, _Held.view(a))
+    return a
 
 
 def quantize_both(x: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> Tuple[Fp8Blocks, Fp8Blocks]:
     """(blocks of x, blocks of x^T) from one read: the second has a scale for each 128 elements of a COLUMN of x."""
-    _format(dtype, "quantize_both")
+    fmt = _format(dtype, "quantize_both")
     _no_graph("quantize_both", x)
     x2, ld = _matrix(x, "quantize_both")
     if x2.shape[0] == 0:
         raise ValueError("quantize_both: a matrix without rows has no columns to cut into blocks")
-    a, b, _ = _quantize(x2, ld, dtype, cols=True)
-    return Fp8Blocks(*a, x2.shape[1]), Fp8Blocks(*b, x2.shape[0])
+    a, b = _new_blocks(*x2.shape, dtype, x.device), _new_blocks(x2.shape[1], x2.shape[0], dtype, x.device)
+    _quantize(x2, ld, fmt, _Held.view(a), _Held.view(b))
+    return a, b
 
 
 def quantize_tiles(w: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> Tuple[Fp8Blocks, Fp8Blocks]:
     """(blocks of w, blocks of w^T) of a weight [out, in] with one scale for each 128 x 128 tile: the two hold the same values."""
-    _format(dtype, "quantize_tiles")
+    fmt = _format(dtype, "quantize_tiles")
     _no_graph("quantize_tiles", w)
     if w.dim() != 2 or w.shape[0] == 0:
         raise ValueError(f"quantize_tiles: a matrix with rows, got {tuple(w.shape)}")
     w2, ld = _matrix(w, "quantize_tiles")
-    a, b, _ = _quantize(w2, ld, dtype, cols=True, tile=True)
-    return Fp8Blocks(*a, w2.shape[1]), Fp8Blocks(*b, w2.shape[0])
+    a, b = _new_blocks(*w2.shape, dtype, w.device), _new_blocks(w2.shape[1], w2.shape[0], dtype, w.device)
+    _quantize(w2, ld, fmt, _Held.view(a), _Held.view(b), tile=True)
+    return a, b
 
 
-def _matmul(a_data, a_scale, b_data, b_scale, K, bias, relu, out_dtype):
-    M, N = a_data.shape[0], b_data.shape[0]
-    dev = a_data.device
+def _matmul(a: _Held, b: _Held, dev, bias, relu, out_dtype):
+    M, N, K = a.rows, b.rows, a.cols
     out = torch.empty((M, N), dtype=out_dtype, device=dev)
     if M == 0 or N == 0:
         return out
@@ -156,12 +185,8 @@ def _matmul(a_data, a_scale, b_data, b_scale, K, bias, relu, out_dtype):
     od = _ROW_DT[out_dtype]
     nbytes = lib.snipper_fp8_matmul_workspace_bytes(M, N, K, od)
     ws = torch.empty(nbytes // 4, dtype=torch.float32, device=dev) if nbytes else None
-    with _lib.device_guard(dev):
-        rc = lib.snipper_fp8_matmul(
-            _lib.raw_stream(dev), a_data.data_ptr(), a_scale.data_ptr(), _FMT[a_data.dtype], b_data.data_ptr(), b_scale.data_ptr(),
-            _FMT[b_data.dtype], M, N, K, bias.data_ptr() if bias is not None else None, _ROW_DT[bias.dtype] if bias is not None else 0,
-            relu, out.data_ptr(), od, ws.data_ptr() if nbytes else None, nbytes)
-    _lib.check(rc, "snipper_fp8_matmul")
+    _call(lib.snipper_fp8_matmul, dev, a.data, a.scale, a.fmt, b.data, b.scale, b.fmt, M, N, K, _opt(bias),
+          _ROW_DT[bias.dtype] if bias is not None else 0, relu, out.data_ptr(), od, _opt(ws), nbytes)
     return out
 
 
@@ -178,18 +203,20 @@ def matmul_fp8(a: Fp8Blocks, b: Fp8Blocks, bias: Optional[torch.Tensor] = None, 
     result's own rounding); a float32 result from the bfloat16 ones on exactly widened operands, at a quarter of the rate."""
     if a.cols != b.cols:
         raise ValueError(f"matmul_fp8: a {a.shape} and b {b.shape} have rows of different length")
-    if not a.data.is_cuda:
+    dev = a.data.device
+    if dev.type != "cuda":
         raise RuntimeError("matmul_fp8: Not implemented on the CPU")
-    if a.data.device != b.data.device:
+    if dev != b.data.device:
         raise ValueError("matmul_fp8: operands on one device")
     if out_dtype not in _ROW_DT:
         raise TypeError(f"matmul_fp8: out_dtype float32, bfloat16 or float16, got {out_dtype}")
-    if max(a.shape[0], b.shape[0], a.cols) > _MAX_DIM:
+    ha, hb = _Held.view(a), _Held.view(b)
+    if ha.rows > _MAX_DIM or hb.rows > _MAX_DIM or a.cols > _MAX_DIM:
         raise ValueError("matmul_fp8: sizes up to 2^23")
     if bias is not None:
         _no_graph("matmul_fp8", bias)
-        _check_bias(bias, b.data.shape[0], a.data.device, "matmul_fp8")
-    return _matmul(a.data, a.scale, b.data, b.scale, a.cols, bias, int(relu), out_dtype)
+        _check_bias(bias, hb.rows, dev, "matmul_fp8")
+    return _matmul(ha, hb, dev, bias, int(relu), out_dtype)
 
 
 def _linear_params(x, weight, bias, what):
@@ -201,49 +228,74 @@ def _linear_params(x, weight, bias, what):
         _check_bias(bias, weight.shape[0], x.device, what)
 
 
-def _linear_backward(ctx, g2, xt, wt, K, x_dtype, want, grad_dtype):
-    """(dx [M, K] or None, dW or None, db or None) from the gradient [M, N]; want = which."""
+def _linear_forward(ctx, x2, ld, weight, bias, out_dtype, want_wt, want_xt, what, norm=None):
+    """y [M, N] of x2 [M, K] (normalised first with ``norm``); keeps on ctx what the backward pass reads: the columns' blocks of the
+    input (for dW) and of the weight (for dx)."""
+    w2, ldw = _matrix(weight, what)
+    M, K = x2.shape
+    N = w2.shape[0]
+    dev = x2.device
+    wr = _Held.new(N, K, 0, dev)
+    wt = _Held.new(K, N, 0, dev) if want_wt else None
+    _quantize(w2, ldw, 0, wr, wt, tile=True)
+    xr = _Held.new(M, K, 0, dev)
+    xt = _Held.new(K, M, 0, dev) if want_xt else None
+    if norm is None:
+        _quantize(x2, ld, 0, xr, xt)
+    else:
+        stats, gamma, beta, p_dtype, eps = norm
+        if want_xt:                                    # both forms: statistics first, then one more read normalises and rounds
+            _layer_norm_forward(x2, ld, gamma, beta, p_dtype, eps, None, stats)
+            _quantize(x2, ld, 0, xr, xt, norm=(stats, gamma, beta, p_dtype))
+        else:
+            _layer_norm_forward(x2, ld, gamma, beta, p_dtype, eps, None, stats, (xr.data, xr.scale))
+    return _matmul(xr, wr, dev, bias, 0, out_dtype), (xt.keep if want_xt else None), (wt.keep if want_wt else None)
+
+
+def _linear_backward(g, dims, xt, wt, dtypes, want, grad_fmt):
+    """(dx [M, K] or None, dW or None, db or None) from the gradient [..., N]; dims (M, N, K); want = which; dtypes of the three."""
+    M, N, K = dims
     wx, ww, wb = want
-    gr, gt, db = _quantize(g2, g2.stride(0) if g2.shape[0] > 1 else g2.shape[1], grad_dtype, rows=wx, cols=ww or not wx, colsum=wb)
-    dx = _matmul(*gr, *wt, g2.shape[1], None, 0, x_dtype) if wx else None
-    dw = _matmul(*gt, *xt, g2.shape[0], None, 0, ctx.param_dtypes[0]) if ww else None
-    return dx, dw, db.to(ctx.param_dtypes[1]) if wb else None
+    g2, ld = _matrix(g if g.dim() == 2 else g.reshape(M, N), "linear_fp8")
+    dev = g2.device
+    gr = _Held.new(M, N, grad_fmt, dev) if wx else None
+    gt = _Held.new(N, M, grad_fmt, dev) if ww or not wx else None
+    db = _quantize(g2, ld, grad_fmt, gr, gt, colsum=wb)
+    dx = _matmul(gr, _Held.of(wt, K, N, 0), dev, None, 0, dtypes[0]) if wx else None
+    dw = _matmul(gt, _Held.of(xt, K, M, 0), dev, None, 0, dtypes[1]) if ww else None
+    return dx, dw, db.to(dtypes[2]) if wb else None
+
+
+def _zero_grads(g, shapes, dtypes, want):
+    return tuple(g.new_zeros(s, dtype=d) if w else None for s, d, w in zip(shapes, dtypes, want))
 
 
 class LinearFp8(Function):
-    """apply(x, weight, bias, grad_dtype): see ``linear_fp8``."""
+    """apply(x, weight, bias, grad_fmt): see ``linear_fp8``."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, grad_dtype):
+    def forward(ctx, x, weight, bias, grad_fmt):
         x2, ld = _matrix(x, "linear_fp8")
-        w2, ldw = _matrix(weight, "linear_fp8")
         M, K = x2.shape
-        N = w2.shape[0]
-        nx, nw, nb = ctx.needs_input_grad[:3]
-        ctx.param_dtypes = (weight.dtype, bias.dtype if bias is not None else None)
-        ctx.dims, ctx.grad_dtype, ctx.x_dtype = (M, N, K), grad_dtype, x.dtype
+        N = weight.shape[0]
+        ctx.meta = (M, N, K), (x.dtype, weight.dtype, bias.dtype if bias is not None else None), grad_fmt, x.shape
         if M == 0:
             ctx.save_for_backward()
             return x.new_empty((*x.shape[:-1], N))
-        wr, wt, _ = _quantize(w2, ldw, torch.float8_e4m3fn, cols=nx, tile=True)
-        xr, xt, _ = _quantize(x2, ld, torch.float8_e4m3fn, cols=nw)
-        y = _matmul(*xr, *wr, K, bias, 0, x.dtype)
-        ctx.save_for_backward(*(xt if nw else (None, None)), *(wt if nx else (None, None)))
-        return y.view(*x.shape[:-1], N)
+        y, xt, wt = _linear_forward(ctx, x2, ld, weight, bias, x.dtype, ctx.needs_input_grad[0], ctx.needs_input_grad[1], "linear_fp8")
+        ctx.save_for_backward(xt, wt)
+        return y if x2 is x else y.view(*x.shape[:-1], N)
 
     @staticmethod
-    @once_differentiable
+    @_once_differentiable
     def backward(ctx, g):
-        M, N, K = ctx.dims
-        nx, nw, nb = ctx.needs_input_grad[:3]
-        if M == 0:
-            return (g.new_empty((*g.shape[:-1], K), dtype=ctx.x_dtype) if nx else None,
-                    g.new_zeros((N, K), dtype=ctx.param_dtypes[0]) if nw else None,
-                    g.new_zeros(N, dtype=ctx.param_dtypes[1]) if nb else None, None)
-        saved = ctx.saved_tensors
-        g2, _ = _matrix(g.reshape(M, N), "linear_fp8")
-        dx, dw, db = _linear_backward(ctx, g2, saved[:2], saved[2:], K, ctx.x_dtype, (nx, nw, nb), ctx.grad_dtype)
-        return dx.view(*g.shape[:-1], K) if nx else None, dw, db, None
+        dims, dtypes, grad_fmt, shape = ctx.meta
+        want = ctx.needs_input_grad[:3]
+        if dims[0] == 0:
+            return *_zero_grads(g, (shape, dims[1:], dims[1]), dtypes, want), None
+        xt, wt = ctx.saved_tensors
+        dx, dw, db = _linear_backward(g, dims, xt, wt, dtypes, want, grad_fmt)
+        return dx.view(shape) if dx is not None and len(shape) != 2 else dx, dw, db, None
 
 
 def linear_fp8(x: torch.Tensor, lin: torch.nn.Linear, grad_dtype: torch.dtype = torch.float8_e4m3fn) -> torch.Tensor:
@@ -252,69 +304,61 @@ def linear_fp8(x: torch.Tensor, lin: torch.nn.Linear, grad_dtype: torch.dtype = 
     x [..., K] float32 / bfloat16 / float16 -> [..., N] of x's type; lin's parameters in any of the three, their gradients in theirs.
     y = x W^T + b, dx = g W and dW = g^T x are products of blocks along the axis that each sums over; g is rounded to ``grad_dtype``
     (e4m3, or e5m2 for more range inside a block); db is the sum of the unrounded g."""
-    _format(grad_dtype, "linear_fp8")
-    _linear_params(x, lin.weight, lin.bias, "linear_fp8")
-    return LinearFp8.apply(x, lin.weight, lin.bias, grad_dtype)
+    fmt = _format(grad_dtype, "linear_fp8")
+    weight, bias = lin.weight, lin.bias
+    _linear_params(x, weight, bias, "linear_fp8")
+    return LinearFp8.apply(x, weight, bias, fmt)
 
 
 def layer_norm_fp8(x: torch.Tensor, norm: torch.nn.LayerNorm, dtype: torch.dtype = torch.float8_e4m3fn) -> Fp8Blocks:
     """``norm(x)`` as blocks, rounded once from float32, in one launch: the left operand of ``matmul_fp8`` at inference."""
     fmt = _format(dtype, "layer_norm_fp8")
-    _no_graph("layer_norm_fp8", x, norm.weight, norm.bias)
-    x2, ld, gamma, beta, p_dtype = _norm_rows(x, norm, "layer_norm_fp8")
-    blocks = _empty_blocks(*x2.shape, dtype, x.device)
-    _layer_norm_forward(x2, ld, gamma, beta, p_dtype, norm.eps, None, None, blocks, fmt)
-    return Fp8Blocks(*blocks, x2.shape[1])
+    gamma, beta = norm.weight, norm.bias
+    _no_graph("layer_norm_fp8", x, gamma, beta)
+    x2, ld, p_dtype = _norm_rows(x, gamma, beta, norm.normalized_shape, "layer_norm_fp8")
+    blocks = _new_blocks(*x2.shape, dtype, x.device)
+    _layer_norm_forward(x2, ld, gamma, beta, p_dtype, norm.eps, None, None, (blocks.data.data_ptr(), blocks.scale.data_ptr()), fmt)
+    return blocks
 
 
 class LayerNormLinearFp8(Function):
-    """apply(x, gamma, beta, weight, bias, norm, grad_dtype): see ``layer_norm_linear_fp8``."""
+    """apply(x, gamma, beta, weight, bias, normalized_shape, eps, grad_fmt): see ``layer_norm_linear_fp8``."""
 
     @staticmethod
-    def forward(ctx, x, gamma, beta, weight, bias, norm, grad_dtype):
+    def forward(ctx, x, gamma, beta, weight, bias, normalized_shape, eps, grad_fmt):
         what = "layer_norm_linear_fp8"
-        x2, ld, gamma, beta, p_dtype = _norm_rows(x, norm, what)
-        w2, ldw = _matrix(weight, what)
+        x2, ld, p_dtype = _norm_rows(x, gamma, beta, normalized_shape, what)
         M, K = x2.shape
-        N = w2.shape[0]
+        N = weight.shape[0]
         if M > _MAX_DIM:
             raise ValueError(f"{what}: up to 2^23 rows")
         nx, ng, nbt, nw, nb = ctx.needs_input_grad[:5]
-        ctx.param_dtypes = (weight.dtype, bias.dtype if bias is not None else None)
-        ctx.dims, ctx.grad_dtype, ctx.p_dtype, ctx.ld = (M, N, K), grad_dtype, p_dtype, ld
+        ctx.meta = (M, N, K), (x.dtype, p_dtype, p_dtype, weight.dtype, bias.dtype if bias is not None else None), grad_fmt, x.shape, ld
         if M == 0:
-            ctx.x_dtype = x.dtype
             ctx.save_for_backward()
             return x.new_empty((*x.shape[:-1], N))
         before = nx or ng or nbt                       # something in front of the product wants a gradient
-        wr, wt, _ = _quantize(w2, ldw, torch.float8_e4m3fn, cols=before, tile=True)
         stats = torch.empty((2, M), dtype=torch.float32, device=x.device) if before or nw else None
-        if nw:                                         # both forms: statistics first, then one more read normalises and rounds
-            _layer_norm_forward(x2, ld, gamma, beta, p_dtype, norm.eps, None, stats)
-            xr, xt, _ = _quantize(x2, ld, torch.float8_e4m3fn, cols=True, norm=(stats, gamma, beta, p_dtype))
-        else:
-            xr, xt = _empty_blocks(M, K, torch.float8_e4m3fn, x.device), (None, None)
-            _layer_norm_forward(x2, ld, gamma, beta, p_dtype, norm.eps, None, stats, xr)
-        y = _matmul(*xr, *wr, K, bias, 0, x.dtype)
-        ctx.save_for_backward(*xt, *(wt if before else (None, None)), x2 if before else None, stats, gamma)
-        return y.view(*x.shape[:-1], N)
+        y, xt, wt = _linear_forward(ctx, x2, ld, weight, bias, x.dtype, before, nw, what, (stats, gamma, beta, p_dtype, eps))
+        ctx.save_for_backward(xt, wt, *((x2, stats, gamma) if before else (None, None, None)))
+        return y if x2 is x else y.view(*x.shape[:-1], N)
 
     @staticmethod
-    @once_differentiable
+    @_once_differentiable
     def backward(ctx, g):
-        M, N, K = ctx.dims
-        nx, ng, nbt, nw, nb = ctx.needs_input_grad[:5]
+        dims, dtypes, grad_fmt, shape, ld = ctx.meta
+        M, N, K = dims
+        want = ctx.needs_input_grad[:5]
         if M == 0:
-            z = lambda want, shape, dtype: g.new_zeros(shape, dtype=dtype) if want else None
-            return (z(nx, (*g.shape[:-1], K), ctx.x_dtype), z(ng, K, ctx.p_dtype), z(nbt, K, ctx.p_dtype),
-                    z(nw, (N, K), ctx.param_dtypes[0]), z(nb, N, ctx.param_dtypes[1]), None, None)
-        *blocks, x2, stats, gamma = ctx.saved_tensors
+            return *_zero_grads(g, (shape, K, K, (N, K), N), dtypes, want), None, None, None
+        nx, ng, nbt, nw, nb = want
+        xt, wt, x2, stats, gamma = ctx.saved_tensors
         before = nx or ng or nbt
-        g2, _ = _matrix(g.reshape(M, N), "layer_norm_linear_fp8")
-        x_dtype = x2.dtype if before else None
-        dz, dw, db = _linear_backward(ctx, g2, blocks[:2], blocks[2:], K, x_dtype, (before, nw, nb), ctx.grad_dtype)
-        dx, dp = _layer_norm_backward(dz, x2, ctx.ld, stats, gamma, ctx.p_dtype, nx, ng or nbt) if before else (None, None)
-        return (dx.view(*g.shape[:-1], K) if nx else None, dp[0] if ng else None, dp[1] if nbt else None, dw, db, None, None)
+        dz, dw, db = _linear_backward(g, dims, xt, wt, (dtypes[0], dtypes[3], dtypes[4]), (before, nw, nb), grad_fmt)
+        dx = dgamma = dbeta = None
+        if before:
+            dx, dgamma, dbeta = _layer_norm_backward(dz, x2, ld, stats, gamma, dtypes[1], nx, ng or nbt)
+        return (dx.view(shape) if nx and len(shape) != 2 else dx, dgamma if ng else None, dbeta if nbt else None, dw, db, None, None, None)
 
 
 def layer_norm_linear_fp8(x: torch.Tensor, norm: torch.nn.LayerNorm, lin: torch.nn.Linear,
@@ -322,6 +366,7 @@ def layer_norm_linear_fp8(x: torch.Tensor, norm: torch.nn.LayerNorm, lin: torch.
     """``lin(norm(x))``, differentiable, as ``linear_fp8`` after ``fused.layer_norm`` without the norm's result in 16 or 32 bits: it is
     rounded from float32 straight into the blocks that the two products read.  The gradient between the two has x's type."""
     what = "layer_norm_linear_fp8"
-    _format(grad_dtype, what)
-    _linear_params(x, lin.weight, lin.bias, what)
-    return LayerNormLinearFp8.apply(x, norm.weight, norm.bias, lin.weight, lin.bias, norm, grad_dtype)
+    fmt = _format(grad_dtype, what)
+    weight, bias = lin.weight, lin.bias
+    _linear_params(x, weight, bias, what)
+    return LayerNormLinearFp8.apply(x, norm.weight, norm.bias, weight, bias, norm.normalized_shape, norm.eps, fmt)

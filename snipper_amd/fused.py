@@ -387,93 +387,116 @@ def ln_fusable(x: torch.Tensor, norm: torch.nn.LayerNorm) -> bool:
 _ROW_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 3}      # include/snipper_fp8.h
 
 
-def _norm_rows(x: torch.Tensor, norm: torch.nn.LayerNorm, what: str):
-    """(x as [rows, C] with unit stride inside a row, row stride, gamma, beta, parameter type) of a layer norm over x's last axis."""
-    if not x.is_cuda:
-        raise RuntimeError(f"{what}: Not implemented on the CPU")
-    if x.dim() < 1 or tuple(norm.normalized_shape) != (x.shape[-1],):
-        raise ValueError(f"{what}: normalized_shape {tuple(norm.normalized_shape)} is not the last axis of {tuple(x.shape)}")
-    C = x.shape[-1]
-    if not 1 <= C <= 16384:
-        raise ValueError(f"{what}: rows of 1 to 16384 elements, got {C}")
-    if x.dtype not in _ROW_DT:
-        raise TypeError(f"{what}: float32, bfloat16 or float16, got {x.dtype}")
-    gamma, beta = norm.weight, norm.bias
-    p_dtype = x.dtype
-    for p in (gamma, beta):
-        if p is not None:
-            if p.dtype not in _ROW_DT or p.device != x.device or not p.is_contiguous():
-                raise TypeError(f"{what}: parameters are contiguous, of a floating type, on x's device")
-            p_dtype = p.dtype
-    if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
-        raise TypeError(f"{what}: weight and bias of one type")
-    x2 = x if x.dim() == 2 else x.reshape(-1, C)
-    if x2.stride(1) != 1 or (x2.shape[0] > 1 and x2.stride(0) < C):
-        x2 = x2.contiguous()
-    if x2.shape[0] >= 2 ** 31:
-        raise ValueError(f"{what}: fewer than 2^31 rows")
-    return x2, (x2.stride(0) if x2.shape[0] > 1 else C), gamma, beta, p_dtype
+def _call(fn, device, *args) -> None:
+    """fn(current stream of ``device``, *args) with that device current; raises on an error code."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(torch._C._cuda_getCurrentRawStream(index), *args)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(_stream(device), *args)
+    if rc:
+        _lib.check(rc, fn.__name__)
+
+
+def _once_differentiable(backward):
+    """``once_differentiable``, at no cost where it matters: a backward pass that builds no graph runs without gradients already."""
+    checked = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 def _opt(t):
     return t.data_ptr() if t is not None else None
 
 
-def _layer_norm_forward(x2, ld, gamma, beta, p_dtype, eps, y, stats, blocks=None, fmt=0):
-    """One launch of snipper_layernorm_forward; nothing for a matrix without rows."""
-    if x2.shape[0] == 0:
+def _norm_rows(x: torch.Tensor, gamma, beta, normalized_shape, what: str):
+    """(x as [rows, C] with unit stride inside a row, row stride, parameter type) of a layer norm over x's last axis."""
+    if not x.is_cuda:
+        raise RuntimeError(f"{what}: Not implemented on the CPU")
+    shape = x.shape
+    if not shape or tuple(normalized_shape) != (shape[-1],):
+        raise ValueError(f"{what}: normalized_shape {tuple(normalized_shape)} is not the last axis of {tuple(shape)}")
+    C = shape[-1]
+    if not 1 <= C <= 16384:
+        raise ValueError(f"{what}: rows of 1 to 16384 elements, got {C}")
+    p_dtype = x.dtype
+    if p_dtype not in _ROW_DT:
+        raise TypeError(f"{what}: float32, bfloat16 or float16, got {x.dtype}")
+    for p in (gamma, beta):
+        if p is not None:
+            p_dtype = p.dtype
+            if p_dtype not in _ROW_DT or p.device != x.device or not p.is_contiguous():
+                raise TypeError(f"{what}: parameters are contiguous, of a floating type, on x's device")
+    if gamma is not None and beta is not None and gamma.dtype is not beta.dtype:
+        raise TypeError(f"{what}: weight and bias of one type")
+    x2 = x if len(shape) == 2 else x.reshape(-1, C)
+    R = x2.shape[0]
+    if R >= 2 ** 31:
+        raise ValueError(f"{what}: fewer than 2^31 rows")
+    ld, inner = x2.stride()
+    if R <= 1 and inner == 1:
+        return x2, C, p_dtype
+    if inner != 1 or ld < C:
+        x2, ld = x2.contiguous(), C
+    return x2, ld, p_dtype
+
+
+def _layer_norm_forward(x2, ld, gamma, beta, p_dtype, eps, y, stats, blocks=(None, None), fmt=0):
+    """One launch of snipper_layernorm_forward; nothing for a matrix without rows.  stats [2, rows]: mean, rstd."""
+    R, C = x2.shape
+    if R == 0:
         return
+    mean = stats.data_ptr() if stats is not None else None
+    _call(_lib.load().snipper_layernorm_forward, x2.device, x2.data_ptr(), _ROW_DT[x2.dtype], ld, _opt(gamma), _opt(beta), _ROW_DT[p_dtype],
+          R, C, eps, _opt(y), mean, mean + 4 * R if mean is not None else None, blocks[0], blocks[1], fmt)
+
+
+def _layer_norm_backward(g, x2, ld, stats, gamma, p_dtype, want_dx, want_params):
+    """(dx [rows, C], dgamma, dbeta) from g, contiguous and of x2's type; None for what is not wanted."""
+    R, C = x2.shape
     dev = x2.device
-    with _lib.device_guard(dev):
-        rc = _lib.load().snipper_layernorm_forward(
-            _stream(dev), x2.data_ptr(), _ROW_DT[x2.dtype], ld, _opt(gamma), _opt(beta), _ROW_DT[p_dtype], x2.shape[0], x2.shape[1],
-            float(eps), _opt(y), stats[0].data_ptr() if stats is not None else None, stats[1].data_ptr() if stats is not None else None,
-            blocks[0].data_ptr() if blocks is not None else None, blocks[1].data_ptr() if blocks is not None else None, fmt)
-    _lib.check(rc, "snipper_layernorm_forward")
-
-
-def _layer_norm_backward(g2, x2, ld, stats, gamma, p_dtype, want_dx, want_params):
-    """(dx like g2 or None, (dgamma, dbeta) or None)."""
-    R, C = g2.shape
-    dev = g2.device
     dx = torch.empty((R, C), dtype=x2.dtype, device=dev) if want_dx else None
-    dp = torch.empty((2, C), dtype=p_dtype, device=dev) if want_params else None
     if not want_params and (R == 0 or not want_dx):
-        return dx, dp
+        return dx, None, None
     lib = _lib.load()
-    nbytes = lib.snipper_layernorm_backward_workspace_bytes(R, C) if want_params else 0
-    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=dev) if nbytes else None
-    with _lib.device_guard(dev):
-        rc = lib.snipper_layernorm_backward(
-            _stream(dev), g2.data_ptr(), x2.data_ptr(), _ROW_DT[x2.dtype], ld, stats[0].data_ptr(), stats[1].data_ptr(), _opt(gamma),
-            _ROW_DT[p_dtype], R, C, _opt(dx), dp[0].data_ptr() if want_params else None, dp[1].data_ptr() if want_params else None,
-            _opt(ws), nbytes)
-    _lib.check(rc, "snipper_layernorm_backward")
-    return dx, dp
+    dgamma = dbeta = ws = None
+    nbytes = 0
+    if want_params:
+        dgamma, dbeta = torch.empty(C, dtype=p_dtype, device=dev), torch.empty(C, dtype=p_dtype, device=dev)
+        nbytes = lib.snipper_layernorm_backward_workspace_bytes(R, C)
+        ws = torch.empty(nbytes // 4, dtype=torch.float32, device=dev) if nbytes else None
+    mean = stats.data_ptr()
+    _call(lib.snipper_layernorm_backward, dev, g.data_ptr(), x2.data_ptr(), _ROW_DT[x2.dtype], ld, mean, mean + 4 * R, _opt(gamma),
+          _ROW_DT[p_dtype], R, C, _opt(dx), _opt(dgamma), _opt(dbeta), _opt(ws), nbytes)
+    return dx, dgamma, dbeta
 
 
 class LayerNormRows(Function):
-    """apply(x, gamma, beta, norm): see ``layer_norm``."""
+    """apply(x, gamma, beta, normalized_shape, eps): see ``layer_norm``."""
 
     @staticmethod
-    def forward(ctx, x, gamma, beta, norm):
-        x2, ld, gamma, beta, p_dtype = _norm_rows(x, norm, "layer_norm")
+    def forward(ctx, x, gamma, beta, normalized_shape, eps):
+        x2, ld, p_dtype = _norm_rows(x, gamma, beta, normalized_shape, "layer_norm")
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        need = any(ctx.needs_input_grad[:3])
-        stats = torch.empty((2, x2.shape[0]), dtype=torch.float32, device=x.device) if need else None
-        _layer_norm_forward(x2, ld, gamma, beta, p_dtype, norm.eps, y, stats)
-        ctx.p_dtype, ctx.ld = p_dtype, ld
+        stats = torch.empty((2, x2.shape[0]), dtype=torch.float32, device=x.device)
+        _layer_norm_forward(x2, ld, gamma, beta, p_dtype, eps, y, stats)
+        ctx.meta = p_dtype, ld, x.shape
         ctx.save_for_backward(x2, stats, gamma)
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once_differentiable
     def backward(ctx, g):
         x2, stats, gamma = ctx.saved_tensors
+        p_dtype, ld, shape = ctx.meta
         wx, wg, wb = ctx.needs_input_grad[:3]
-        g2 = g.to(x2.dtype).contiguous().view(x2.shape)
-        dx, dp = _layer_norm_backward(g2, x2, ctx.ld, stats, gamma, ctx.p_dtype, wx, wg or wb)
-        return dx.view(g.shape) if wx else None, dp[0] if wg else None, dp[1] if wb else None, None
+        if g.dtype is not x2.dtype or not g.is_contiguous():
+            g = g.to(x2.dtype).contiguous()
+        dx, dgamma, dbeta = _layer_norm_backward(g, x2, ld, stats, gamma, p_dtype, wx, wg or wb)
+        return dx.view(shape) if wx and len(shape) != 2 else dx, dgamma if wg else None, dbeta if wb else None, None, None
 
 
 def layer_norm(x: torch.Tensor, norm: torch.nn.LayerNorm) -> torch.Tensor:
@@ -481,7 +504,13 @@ def layer_norm(x: torch.Tensor, norm: torch.nn.LayerNorm) -> torch.Tensor:
     take: rows of any width up to 16384, any row stride, float16 beside float32 and bfloat16, an ``nn.LayerNorm`` without weight or
     bias.  The result and dx have x's type, dgamma and dbeta the parameters' (which is x's or another of the three); statistics and
     sums are float32, dgamma and dbeta are summed in a fixed order."""
-    return LayerNormRows.apply(x, norm.weight, norm.bias, norm)
+    gamma, beta = norm.weight, norm.bias
+    if torch.is_grad_enabled() and (x.requires_grad or (gamma is not None and gamma.requires_grad) or (beta is not None and beta.requires_grad)):
+        return LayerNormRows.apply(x, gamma, beta, norm.normalized_shape, norm.eps)
+    x2, ld, p_dtype = _norm_rows(x, gamma, beta, norm.normalized_shape, "layer_norm")
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _layer_norm_forward(x2, ld, gamma, beta, p_dtype, norm.eps, y, None)
+    return y
 
 
 class InputProjTokens(Function):
