@@ -81,7 +81,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(NORM ? 5 : 
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const long long r = row_of(k) < a.R ? row_of(k) : a.R - 1;
-      load8((const T *)a.x + r * a.ldx + c, 8, v[k]);
+      load_w<8, true>((const T *)a.x + r * a.ldx + c, 8, v[k]);        // (past the caches: what comes out is what is read again)
     }
   } else {
 #pragma unroll

@@ -18,11 +18,17 @@ enum { kF32 = 0, kBF16 = 1, kF16 = 3 };           // type codes of the C ABI
 // W consecutive elements of a row as float.  The address needs no more than the element's own alignment: memory instructions take any
 // on this hardware (a piece that straddles a cache line costs one more access), so odd widths and strides run the same code as even
 // ones.  `n` elements exist (n >= W: all); the others read as 0.
-template <int W, typename T>
+template <int W, bool NT = false, typename T>
 __device__ __forceinline__ void load_w(const T *p, int n, float (&v)[W]) {
   if (n >= W) {
     T t[W];
-    __builtin_memcpy(t, p, W * sizeof(T));
+    if constexpr (NT) {
+      typedef unsigned U __attribute__((ext_vector_type(W * sizeof(T) / 4), aligned(sizeof(T))));
+      const U u = __builtin_nontemporal_load((const U *)p);
+      __builtin_memcpy(t, &u, sizeof(u));
+    } else {
+      __builtin_memcpy(t, p, W * sizeof(T));
+    }
 #pragma unroll
     for (int j = 0; j < W; ++j) v[j] = (float)t[j];
   } else {
@@ -43,6 +49,21 @@ __device__ __forceinline__ void store_w(T *p, int n, const float (&v)[W]) {
       if (j < n) p[j] = t[j];
   }
 }
+// past the caches
+template <int W, typename T>
+__device__ __forceinline__ void store_nt(T *p, int n, const float (&v)[W]) {
+  if (n >= W) {
+    typedef unsigned V __attribute__((ext_vector_type(W * sizeof(T) / 4), aligned(sizeof(T))));
+    T t[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) t[j] = (T)v[j];
+    V u;
+    __builtin_memcpy(&u, t, sizeof(u));
+    __builtin_nontemporal_store(u, (V *)p);
+  } else {
+    store_w<W>(p, n, v);
+  }
+}
 template <typename T>
 __device__ __forceinline__ void load8(const T *p, int n, float (&v)[8]) { load_w<8>(p, n, v); }
 template <typename T>
@@ -52,9 +73,16 @@ template <typename T, int W>
 struct Raw {
   typedef T V __attribute__((ext_vector_type(W)));
   V v;
+  template <bool NT = false>                      // NT: read for the last time, past the caches
   __device__ __forceinline__ void load(const T *p, int n) {
     if (n >= W) {
-      __builtin_memcpy(&v, p, W * sizeof(T));
+      if constexpr (NT) {
+        typedef unsigned U __attribute__((ext_vector_type(W * sizeof(T) / 4), aligned(sizeof(T))));
+        const U u = __builtin_nontemporal_load((const U *)p);
+        __builtin_memcpy(&v, &u, sizeof(u));
+      } else {
+        __builtin_memcpy(&v, p, W * sizeof(T));
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < W; ++j) v[j] = j < n ? p[j] : (T)0.f;
