@@ -221,7 +221,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mm_tile_kernel(MmArgs a) {
   const int key_b = (r & 3) | (r & 4);                          // bit 3 of mm_pair_row(., r) is bit 2 of r
   auto step = [&](auto sel_c, int kt) {
     constexpr int SEL = decltype(sel_c)::value;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    wait_loads<0>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     if (kt + 1 < k_end) {
@@ -243,6 +243,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mm_tile_kernel(MmArgs a) {
       read_frag(base + (BM + wn * TN * 16 + mm_pair_row(j, r)) * 128, key_b, lo, hi);
       b[j].set(lo, hi, sb[j], SEL);
     }
+    if constexpr (EXACT) __builtin_amdgcn_s_setprio(1);         // (the wave beside this one widens meanwhile: 274 -> 269 us of a training step)
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       i32x4 lo, hi;
@@ -252,6 +253,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mm_tile_kernel(MmArgs a) {
 #pragma unroll
       for (int j = 0; j < TN; ++j) acc[i][j] = mm_step<FB, FA, SEL>(b[j], x, acc[i][j], sb[j], sa[i]);
     }
+    if constexpr (EXACT) __builtin_amdgcn_s_setprio(0);
   };
   if (k_begin < k_end) {
     issue(k_begin, k_begin & 1);

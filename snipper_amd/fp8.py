@@ -8,13 +8,14 @@ What the bf16 products of ``dense.py`` are for Linears in 16 bits, these are in 
     layer_norm_fp8(x, norm)                          ``norm(x)`` straight into blocks, for inference
     layer_norm_linear_fp8(x, norm, lin)              ``lin(norm(x))``, differentiable, the norm's result held in 8 bits only
 
-At inference a weight is laid out once, ``w8, _ = quantize_tiles(lin.weight)``, and used as
+At inference, under ``torch.no_grad()``, a weight is laid out once, ``w8, _ = quantize_tiles(lin.weight)``, and used as
 ``matmul_fp8(quantize_rows(x), w8, lin.bias)`` or ``matmul_fp8(layer_norm_fp8(x, norm), w8, lin.bias)``.
 
 Blocks run along the axis that a product sums over.  The training step therefore rounds x and the gradient twice, along their rows
 (y = x W^T, dx = g W) and along their columns (dW = g^T x), both from one read; a weight has one scale for each 128 x 128 tile, so its
 transpose holds the same values.  Scales are powers of two that keep the largest element of a block in range: nothing saturates, and
-an element is its input rounded once.  CUDA tensors only, as everywhere in this package.
+an element is its input rounded once.  CUDA tensors only, as everywhere in this package; autocast changes nothing here, a result has
+x's type.
 """
 from __future__ import annotations
 

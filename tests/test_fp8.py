@@ -107,6 +107,7 @@ def test_c_matmul_refuses():
     for bad in (dict(M=0), dict(N=0), dict(K=0), dict(K=(1 << 23) + 1), dict(fa=2), dict(fb=-1), dict(odt=2), dict(bdt=2),
                 dict(a=ctypes.c_void_p(4104)), dict(sb=ctypes.c_void_p(4098))):
         assert call(**bad) == SHAPE, bad
+    assert call(M=1 << 23, N=1 << 17) == SHAPE                                # (2^40 elements of a result)
     need = lib.snipper_fp8_matmul_workspace_bytes(384, 1024, 79000, 0)         # (a weight gradient: the reduction is split)
     assert need > 0 and need % (384 * 1024 * 4) == 0
     assert call(M=384, N=1024, K=79000, odt=0) == SHAPE and call(M=384, N=1024, K=79000, odt=0, ws=P, nb=need - 1) == SHAPE
@@ -125,6 +126,7 @@ def test_c_layer_norm_refuses():
     for bad in (dict(rows=0), dict(cols=0), dict(cols=16385, ld=16385), dict(ld=100), dict(dt=2), dict(pdt=4), dict(fmt=3), dict(eps=-1.0),
                 dict(eps=float("nan")), dict(d=ctypes.c_void_p(4100), s=P)):
         assert fwd(**bad) == SHAPE, bad
+    assert lib.snipper_layernorm_backward_workspace_bytes((1 << 31) - 1, 100) > 0       # (the largest number of rows)
     assert bwd(g=None) == NULL and bwd(mean=None) == NULL and bwd(dx=None) == NULL and bwd(dg=P) == NULL
     need = lib.snipper_layernorm_backward_workspace_bytes(4, 200)
     assert need == 2 * 200 * 4

@@ -428,3 +428,74 @@ def test_two_captured_graphs_replayed_in_turn():
             torch.cuda.synchronize()
             for a, b in zip(outs[i], step(x[i])):
                 assert torch.equal(a, b)
+
+
+def test_threads_at_once():
+    """Two threads on streams of their own: the library keeps nothing between calls."""
+    import threading
+    lin, norm = _linear(130, 200, torch.float32), _norm(200)
+    xs = [_x(257, 200, torch.bfloat16, seed=s, spread=0.3) for s in (1, 2)]
+    g = torch.randn(257, 130, generator=_gen(7)).bfloat16().to(DEV)
+
+    def step(x):
+        x = x.detach().requires_grad_()
+        y = fp8.layer_norm_linear_fp8(x, norm, lin)
+        return (y.detach(),) + torch.autograd.grad(y, (x, norm.weight, norm.bias, lin.weight, lin.bias), g)
+    want = [step(x) for x in xs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def loop(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                got = step(xs[i])
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    bad.append(i)
+    threads = [threading.Thread(target=loop, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_second_derivatives_are_refused():
+    x, lin, norm = _x(20, 72, torch.float32, spread=0.3).requires_grad_(), _linear(48, 72, torch.float32), _norm(72)
+    for f in (lambda: fp8.linear_fp8(x, lin), lambda: fp8.layer_norm_linear_fp8(x, norm, lin), lambda: fused.layer_norm(x, norm)):
+        y = f()
+        first = torch.autograd.grad(y.sum(), x)[0]
+        graph = torch.autograd.grad(f().square().sum(), x, create_graph=True)[0]
+        assert graph.shape == first.shape
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            graph.sum().backward()
+
+
+def test_rows_of_blocks_and_one_matrix_on_both_sides():
+    """A run of rows of blocks is blocks again; a product of a matrix with itself is symmetric."""
+    x = _x(300, 700, torch.float32, spread=0.3)
+    a = fp8.quantize_rows(x)
+    part = fp8.Fp8Blocks(a.data[37:201], a.scale[37:201], 700)
+    for out in (torch.bfloat16, torch.float32):
+        y = fp8.matmul_fp8(a, a, out_dtype=out)
+        assert torch.equal(y, y.t())
+        _check_product(fp8.matmul_fp8(part, a, out_dtype=out), part, a, None, False, out)
+
+
+def test_autocast_and_inference_mode_change_nothing():
+    x, lin = _x(33, 72, torch.float32, spread=0.3), _linear(48, 72, torch.float32)
+    with torch.no_grad():
+        y = fp8.linear_fp8(x, lin)
+        with torch.autocast("cuda", torch.bfloat16):
+            z = fp8.linear_fp8(x, lin)
+    assert y.dtype == z.dtype == torch.float32 and torch.equal(y, z)
+    with torch.inference_mode():
+        assert torch.equal(fp8.linear_fp8(x, lin), y)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_another_device_than_the_current_one():
+    x, lin = _x(33, 72, torch.float32, spread=0.3).to("cuda:1").requires_grad_(), _linear(48, 72, torch.float32).to("cuda:1")
+    with torch.cuda.device(0):
+        fp8.linear_fp8(x, lin).sum().backward()
+    assert x.grad.device == x.device and torch.isfinite(x.grad).all()
