@@ -33,7 +33,8 @@ extern "C" {
  * if data_t is given, for each 128 elements of a column (data_t / scale_t: the blocks of the transposed matrix [cols][rows]).
  * tile_rows = 128: one scale for each 128 x 128 tile, the same in both forms.  Either form may be NULL, not both.
  * mean / rstd [rows] float32 (or both NULL): x is normalised first, (x - mean) * rstd * gamma + beta, gamma / beta [cols] of type
- * p_dtype or NULL (1 / 0).
+ * p_dtype or NULL (1 / 0); with tile_rows = 1 only.
+ * Data pointers 16-byte, scale pointers 4-byte aligned.
  * colsum [cols] float32 or NULL: the sums of x over the rows, unrounded; needs snipper_fp8_quantize_workspace_bytes of workspace
  * (0 without it).  rows, cols <= 2^23. */
 size_t snipper_fp8_quantize_workspace_bytes(int rows, int cols, int with_colsum);
@@ -43,7 +44,7 @@ int snipper_fp8_quantize(void *stream, const void *x, int x_dtype, long long ldx
                          void *workspace, size_t workspace_bytes);
 
 /* out [M][N] = act(A [M][K] . B [N][K]^T + bias [N]) of two matrices in blocks; act = ReLU if relu, bias of type bias_dtype or NULL.
- * data pointers 16-byte, scale pointers 4-byte aligned.  out [M][N] contiguous, of type out_dtype.
+ * A, B and out 16-byte, scale pointers 4-byte aligned.  out [M][N] contiguous, of type out_dtype.
  * A bfloat16 / float16 result comes from the 8-bit matrix instructions, which align the products of a block to their largest and
  * drop what lies 2^13 below it (1.5e-5 of the result's norm, whatever K); a float32 result comes from the bfloat16 ones on exactly
  * converted operands (1e-7; magnitudes under 2^-126 count as zero there), at a quarter of the rate.  M, N, K <= 2^23, M N < 2^40. */

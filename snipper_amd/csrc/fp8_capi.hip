@@ -42,24 +42,34 @@ void with_fmt(int fmt, F &&f) {
   else f(std::integral_constant<int, 1>{});
 }
 
-// ---- layer norm: lanes of a row and chunks of 8 elements of a lane
-template <typename F>
+// ---- layer norm: lanes of a row and how often eight elements of a lane.  Times in us, forward / backward, of 2^27 bytes (cols x type):
+// 16 lanes share a block of 128 and four rows a wave, one wave a row needs no barrier, four waves a row only one number from each.
+//   256 x 16 bits: 16 lanes 82 / 135, a wave 141 / 231; 384 x 16 bits: 83 / 137 against 104 / 205; but 384 x float32, whose pieces of 16
+//   bytes fill a wave, 89 / 158 against 80 / 133, and 512 x 16 bits 84 / 133 against 86 / 137
+//   2048: four waves 79 / 135 (float32), 83 / 141 (16 bits), a wave 78 / 138, 82 / 137; 4096: four waves 79 / 132, 79 / 140, eight 80 / 131,
+//   86 / 150; 8192: four 79 / 141, 79 / 139, eight 79 / 149, 80 / 173, sixteen 79 / 147, 116 / 171; 16 384: sixteen 84 / 155, 91 / 150,
+//   eight (with all their registers) 91 / 158, 87 / 162
+template <typename T, typename F>
 void with_ln_shape(int cols, F &&f) {
   using std::integral_constant;
-  if (cols <= 128) f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
-  else if (cols <= 512) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+  if (cols <= 128) return f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+  if constexpr (sizeof(T) == 2) {
+    if (cols <= 256) return f(integral_constant<int, 16>{}, integral_constant<int, 2>{});
+    if (cols <= 384) return f(integral_constant<int, 16>{}, integral_constant<int, 3>{});
+  }
+  if (cols <= 512) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
   else if (cols <= 1024) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
   else if (cols <= 2048) f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
-  else if (cols <= 4096) f(integral_constant<int, 512>{}, integral_constant<int, 1>{});
-  else if (cols <= 8192) f(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
+  else if (cols <= 4096) f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+  else if (cols <= 8192) f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
   else f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
 }
-int ln_rows_per_wg(int cols) { return cols <= 128 ? 16 : cols <= 1024 ? 4 : 1; }
-int ln_wgs_per_cu(int cols) { return cols <= 2048 ? 8 : cols <= 4096 ? 4 : 2; }                 // as many as are resident
-int ln_fwd_blocks(int rows, int cols) { return std::min(ceil_div(rows, ln_rows_per_wg(cols)), ln_wgs_per_cu(cols) * kCUs); }
-int ln_bwd_blocks(int rows, int cols) {
-  return std::min(ceil_div(rows, ln_rows_per_wg(cols)), (cols <= 2048 ? 4 : cols <= 8192 ? 2 : 1) * kCUs);
-}
+// Forward: short runs of rows (more workgroups than are resident even out the card's ends: 8 of four waves per CU 84 .. 93, 32 77 .. 83),
+// except that with sixteen waves a row the parameters' loads weigh (2 per CU 91, 8 98).  Backward: every workgroup leaves a row of sums
+// behind, so no more than are resident; fewer for the widest (8192: 4 per CU 147 / 150, 2 141 / 139; 16 384: 2 158, 1 152).
+int ln_fwd_blocks(int rows, int rows_per_wg, int cols) { return std::min(ceil_div(rows, rows_per_wg), (cols <= 8192 ? 32 : 2) * kCUs); }
+int ln_bwd_most(int cols) { return (cols <= 2048 ? 4 : cols <= 8192 ? 2 : 1) * kCUs; }
+int ln_bwd_blocks(int rows, int rows_per_wg, int cols) { return std::min(ceil_div(rows, rows_per_wg), ln_bwd_most(cols)); }
 
 // ---- product: which kernel, and how many pieces the K axis is cut into (times in us of bfloat16 results, M x N x K, 256 CUs)
 struct MmPlan {
@@ -123,7 +133,7 @@ int snipper_fp8_quantize(void *stream, const void *x, int x_dtype, long long ldx
                          uint8_t *scale, uint8_t *data_t, uint8_t *scale_t, float *colsum, void *workspace, size_t workspace_bytes) {
   if (!x || (!data && !data_t) || (data && !scale) || (data_t && !scale_t) || ((mean == nullptr) != (rstd == nullptr))) return SNIPPER_E_NULL;
   if (!dim_ok(rows) || !dim_ok(cols) || ldx < cols || !type_ok(x_dtype) || !type_ok(p_dtype) || !fmt_ok(fmt)) return SNIPPER_E_SHAPE;
-  if (tile_rows != 1 && tile_rows != 128) return SNIPPER_E_SHAPE;
+  if (tile_rows != 1 && (tile_rows != 128 || mean)) return SNIPPER_E_SHAPE;
   if (!mean && (gamma || beta)) return SNIPPER_E_SHAPE;
   if (((uintptr_t)data | (uintptr_t)data_t) & 15 || ((uintptr_t)scale | (uintptr_t)scale_t) & 3) return SNIPPER_E_SHAPE;
   if (colsum && (!workspace || workspace_bytes < snipper_fp8_quantize_workspace_bytes(rows, cols, 1))) return SNIPPER_E_SHAPE;
@@ -143,13 +153,9 @@ int snipper_fp8_quantize(void *stream, const void *x, int x_dtype, long long ldx
     with_fmt(fmt, [&](auto f) {
       using T = decltype(t);
       constexpr int F = decltype(f)::value;
-      if (tile_rows == 128) {
-        if (mean) hipLaunchKernelGGL((quant_tile_kernel<T, F, true, true>), grid, dim3(512), 0, st, a);
-        else hipLaunchKernelGGL((quant_tile_kernel<T, F, true, false>), grid, dim3(512), 0, st, a);
-      } else {
-        if (mean) hipLaunchKernelGGL((quant_tile_kernel<T, F, false, true>), grid, dim3(512), 0, st, a);
-        else hipLaunchKernelGGL((quant_tile_kernel<T, F, false, false>), grid, dim3(512), 0, st, a);
-      }
+      if (tile_rows == 128) hipLaunchKernelGGL((quant_tile_kernel<T, F, true, false>), grid, dim3(512), 0, st, a);
+      else if (mean) hipLaunchKernelGGL((quant_tile_kernel<T, F, false, true>), grid, dim3(512), 0, st, a);
+      else hipLaunchKernelGGL((quant_tile_kernel<T, F, false, false>), grid, dim3(512), 0, st, a);
     });
   });
   if (colsum) hipLaunchKernelGGL(colsum_parts_kernel, dim3(ceil_div(cols, 32)), dim3(1024), 0, st, (const float *)workspace, rb, cols, colsum);
@@ -167,7 +173,7 @@ int snipper_fp8_matmul(void *stream, const uint8_t *A, const uint8_t *a_scale, i
                        void *workspace, size_t workspace_bytes) {
   if (!A || !a_scale || !B || !b_scale || !out) return SNIPPER_E_NULL;
   if (!dim_ok(M) || !dim_ok(N) || !dim_ok(K) || !result_ok(M, N) || !fmt_ok(a_fmt) || !fmt_ok(b_fmt) || !type_ok(out_dtype) || !type_ok(bias_dtype)) return SNIPPER_E_SHAPE;
-  if (((uintptr_t)A | (uintptr_t)B) & 15 || ((uintptr_t)a_scale | (uintptr_t)b_scale) & 3) return SNIPPER_E_SHAPE;
+  if (((uintptr_t)A | (uintptr_t)B | (uintptr_t)out) & 15 || ((uintptr_t)a_scale | (uintptr_t)b_scale) & 3) return SNIPPER_E_SHAPE;
   const bool exact = out_dtype == kF32;
   const MmPlan p = mm_plan(M, N, K, exact);
   const size_t need = snipper_fp8_matmul_workspace_bytes(M, N, K, out_dtype);
@@ -213,12 +219,12 @@ int snipper_layernorm_forward(void *stream, const void *x, int x_dtype, long lon
   LnRowsArgs a{};
   a.x = x; a.ldx = ldx; a.gamma = gamma; a.beta = beta; a.p_dtype = p_dtype; a.R = rows; a.C = cols; a.eps = eps;
   a.y = y; a.mean = mean; a.rstd = rstd; a.data = data; a.scale = scale;
-  const dim3 grid(ln_fwd_blocks(rows, cols));
   hipStream_t st = (hipStream_t)stream;
   with_type(x_dtype, [&](auto t) {
-    with_ln_shape(cols, [&](auto lpr, auto nit) {
-      using T = decltype(t);
+    using T = decltype(t);
+    with_ln_shape<T>(cols, [&](auto lpr, auto nit) {
       constexpr int L = decltype(lpr)::value, I = decltype(nit)::value;
+      const dim3 grid(ln_fwd_blocks(rows, LnShape<T, L, I>::RPW, cols));
       if (!data) hipLaunchKernelGGL((ln_rows_fwd_kernel<T, L, I, -1>), grid, dim3(ln_threads(L)), 0, st, a);
       else if (fmt == 0) hipLaunchKernelGGL((ln_rows_fwd_kernel<T, L, I, 0>), grid, dim3(ln_threads(L)), 0, st, a);
       else hipLaunchKernelGGL((ln_rows_fwd_kernel<T, L, I, 1>), grid, dim3(ln_threads(L)), 0, st, a);
@@ -229,7 +235,7 @@ int snipper_layernorm_forward(void *stream, const void *x, int x_dtype, long lon
 
 size_t snipper_layernorm_backward_workspace_bytes(int rows, int cols) {
   if (rows <= 0 || cols <= 0 || cols > kLnMaxCols) return 0;
-  return (size_t)ln_bwd_blocks(rows, cols) * 2 * cols * sizeof(float);
+  return (size_t)ln_bwd_blocks(rows, cols <= 1024 ? 4 : 1, cols) * 2 * cols * sizeof(float);        // (4: the fewest rows of a workgroup there)
 }
 
 int snipper_layernorm_backward(void *stream, const void *g, const void *x, int x_dtype, long long ldx, const float *mean, const float *rstd,
@@ -239,7 +245,7 @@ int snipper_layernorm_backward(void *stream, const void *g, const void *x, int x
   if (rows < 0 || cols <= 0 || cols > kLnMaxCols || ldx < cols || !type_ok(x_dtype) || !type_ok(p_dtype)) return SNIPPER_E_SHAPE;
   if (rows > 0 && (!g || !x || !mean || !rstd)) return SNIPPER_E_NULL;
   if (rows > 0 && dgamma && (!workspace || workspace_bytes < snipper_layernorm_backward_workspace_bytes(rows, cols))) return SNIPPER_E_SHAPE;
-  const int blocks = rows > 0 ? ln_bwd_blocks(rows, cols) : 0;
+  int blocks = 0;
   LnRowsArgs a{};
   a.x = x; a.ldx = ldx; a.gamma = gamma; a.p_dtype = p_dtype; a.R = rows; a.C = cols;
   a.mean = const_cast<float *>(mean); a.rstd = const_cast<float *>(rstd);
@@ -247,9 +253,11 @@ int snipper_layernorm_backward(void *stream, const void *g, const void *x, int x
   hipStream_t st = (hipStream_t)stream;
   if (rows > 0)
     with_type(x_dtype, [&](auto t) {
-      with_ln_shape(cols, [&](auto lpr, auto nit) {
+      using T = decltype(t);
+      with_ln_shape<T>(cols, [&](auto lpr, auto nit) {
         constexpr int L = decltype(lpr)::value, I = decltype(nit)::value;
-        hipLaunchKernelGGL((ln_rows_bwd_kernel<decltype(t), L, I>), dim3(blocks), dim3(ln_threads(L)), 0, st, a);
+        blocks = ln_bwd_blocks(rows, LnShape<T, L, I>::RPW, cols);
+        hipLaunchKernelGGL((ln_rows_bwd_kernel<T, L, I>), dim3(blocks), dim3(ln_threads(L)), 0, st, a);
       });
     });
   if (dgamma)

@@ -141,7 +141,7 @@ __global__ __launch_bounds__(ln_threads(LPR)) void ln_rows_fwd_kernel(LnRowsArgs
         }
         // the first of a block's lanes writes its byte (127 behind the last block: those blocks are zeros)
         if (in && l % LPB == 0 && (c >> 7) < Q) a.scale[row * Q + (c >> 7)] = (uint8_t)byte;
-        if (LPR == 16 && in && l > 0 && l < 4) a.scale[row * Q + l] = 127;      // (one block: the lanes of the other three are not here)
+        if (LPR == 16 && p == 0 && in && l >= NIT && l < 4) a.scale[row * Q + l] = 127;      // (behind the last block: no lanes there)
       }
     }
   }

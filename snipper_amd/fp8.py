@@ -68,9 +68,8 @@ class _Held:
         self.keep, self.data, self.scale, self.rows, self.cols, self.fmt = keep, data, scale, rows, cols, fmt
 
     @staticmethod
-    def new(rows: int, cols: int, fmt: int, device) -> "_Held":
-        n = rows * (-(-cols // 128) * 128)
-        return _Held.of(torch.empty(n + rows * (-(-cols // 512) * 4), dtype=torch.uint8, device=device), rows, cols, fmt)
+    def new(rows: int, cols: int, fmt: int, like: torch.Tensor) -> "_Held":
+        return _Held.of(like.new_empty(rows * (-(-cols // 128) * 128 + -(-cols // 512) * 4), dtype=torch.uint8), rows, cols, fmt)
 
     @staticmethod
     def of(buf, rows: int, cols: int, fmt: int) -> "_Held":
@@ -124,19 +123,18 @@ def _quantize(x2, ld, fmt, a=None, b=None, tile=False, colsum=False, norm=None):
     """x into a (blocks of x) and / or b (blocks of x^T); the sums over the rows if ``colsum``.  ``norm``: (stats [2, R], gamma, beta,
     p_dtype)."""
     R, C = x2.shape
-    dev = x2.device
     lib = _lib.load()
     s = ws = None
     nbytes = 0
     if colsum:
         nbytes = lib.snipper_fp8_quantize_workspace_bytes(R, C, 1)
-        s, ws = torch.empty(C, dtype=torch.float32, device=dev), torch.empty(nbytes // 4, dtype=torch.float32, device=dev)
+        s, ws = x2.new_empty(C, dtype=torch.float32), x2.new_empty(nbytes // 4, dtype=torch.float32)
     mean = rstd = gamma = beta = None
     p_dtype = 0
     if norm is not None:
         mean, gamma, beta, p_dtype = norm[0].data_ptr(), _opt(norm[1]), _opt(norm[2]), _ROW_DT[norm[3]]
         rstd = mean + 4 * R
-    _call(lib.snipper_fp8_quantize, dev, x2.data_ptr(), _ROW_DT[x2.dtype], ld, R, C, 128 if tile else 1, fmt, mean, rstd, gamma, beta, p_dtype,
+    _call(lib.snipper_fp8_quantize, x2.get_device(), x2.data_ptr(), _ROW_DT[x2.dtype], ld, R, C, 128 if tile else 1, fmt, mean, rstd, gamma, beta, p_dtype,
           a.data if a is not None else None, a.scale if a is not None else None, b.data if b is not None else None,
           b.scale if b is not None else None, _opt(s), _opt(ws), nbytes)
     return s
@@ -177,16 +175,20 @@ def quantize_tiles(w: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn) ->
     return a, b
 
 
-def _matmul(a: _Held, b: _Held, dev, bias, relu, out_dtype):
-    M, N, K = a.rows, b.rows, a.cols
-    out = torch.empty((M, N), dtype=out_dtype, device=dev)
+def _matmul(like: torch.Tensor, a: _Held, b: _Held, bias, out_dtype):
+    return _product(like, a.data, a.scale, a.fmt, b.data, b.scale, b.fmt, a.rows, b.rows, a.cols, bias, 0, out_dtype)
+
+
+def _product(like, a_data, a_scale, a_fmt, b_data, b_scale, b_fmt, M, N, K, bias, relu, out_dtype):
+    """[M, N] on the device of ``like``."""
+    out = like.new_empty((M, N), dtype=out_dtype)
     if M == 0 or N == 0:
         return out
     lib = _lib.load()
     od = _ROW_DT[out_dtype]
     nbytes = lib.snipper_fp8_matmul_workspace_bytes(M, N, K, od)
-    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=dev) if nbytes else None
-    _call(lib.snipper_fp8_matmul, dev, a.data, a.scale, a.fmt, b.data, b.scale, b.fmt, M, N, K, _opt(bias),
+    ws = like.new_empty(nbytes // 4, dtype=torch.float32) if nbytes else None
+    _call(lib.snipper_fp8_matmul, like.get_device(), a_data, a_scale, a_fmt, b_data, b_scale, b_fmt, M, N, K, _opt(bias),
           _ROW_DT[bias.dtype] if bias is not None else 0, relu, out.data_ptr(), od, _opt(ws), nbytes)
     return out
 
@@ -202,22 +204,23 @@ def matmul_fp8(a: Fp8Blocks, b: Fp8Blocks, bias: Optional[torch.Tensor] = None, 
 
     A bfloat16 / float16 result comes from the 8-bit matrix instructions (relative error of their sums 1.5e-5, far inside the
     result's own rounding); a float32 result from the bfloat16 ones on exactly widened operands, at a quarter of the rate."""
-    if a.cols != b.cols:
+    K, ad, bd = a.cols, a.data, b.data
+    if K != b.cols:
         raise ValueError(f"matmul_fp8: a {a.shape} and b {b.shape} have rows of different length")
-    dev = a.data.device
-    if dev.type != "cuda":
+    if not ad.is_cuda:
         raise RuntimeError("matmul_fp8: Not implemented on the CPU")
-    if dev != b.data.device:
+    if ad.get_device() != bd.get_device():
         raise ValueError("matmul_fp8: operands on one device")
     if out_dtype not in _ROW_DT:
         raise TypeError(f"matmul_fp8: out_dtype float32, bfloat16 or float16, got {out_dtype}")
-    ha, hb = _Held.view(a), _Held.view(b)
-    if ha.rows > _MAX_DIM or hb.rows > _MAX_DIM or a.cols > _MAX_DIM:
+    M, N = ad.shape[0], bd.shape[0]
+    if M > _MAX_DIM or N > _MAX_DIM or K > _MAX_DIM:
         raise ValueError("matmul_fp8: sizes up to 2^23")
     if bias is not None:
         _no_graph("matmul_fp8", bias)
-        _check_bias(bias, hb.rows, dev, "matmul_fp8")
-    return _matmul(ha, hb, dev, bias, int(relu), out_dtype)
+        _check_bias(bias, N, ad.device, "matmul_fp8")
+    return _product(ad, ad.data_ptr(), a.scale.data_ptr(), _FMT[ad.dtype], bd.data_ptr(), b.scale.data_ptr(), _FMT[bd.dtype], M, N, K, bias,
+                    int(relu), out_dtype)
 
 
 def _linear_params(x, weight, bias, what):
@@ -235,12 +238,11 @@ def _linear_forward(ctx, x2, ld, weight, bias, out_dtype, want_wt, want_xt, what
     w2, ldw = _matrix(weight, what)
     M, K = x2.shape
     N = w2.shape[0]
-    dev = x2.device
-    wr = _Held.new(N, K, 0, dev)
-    wt = _Held.new(K, N, 0, dev) if want_wt else None
+    wr = _Held.new(N, K, 0, x2)
+    wt = _Held.new(K, N, 0, x2) if want_wt else None
     _quantize(w2, ldw, 0, wr, wt, tile=True)
-    xr = _Held.new(M, K, 0, dev)
-    xt = _Held.new(K, M, 0, dev) if want_xt else None
+    xr = _Held.new(M, K, 0, x2)
+    xt = _Held.new(K, M, 0, x2) if want_xt else None
     if norm is None:
         _quantize(x2, ld, 0, xr, xt)
     else:
@@ -250,7 +252,7 @@ def _linear_forward(ctx, x2, ld, weight, bias, out_dtype, want_wt, want_xt, what
             _quantize(x2, ld, 0, xr, xt, norm=(stats, gamma, beta, p_dtype))
         else:
             _layer_norm_forward(x2, ld, gamma, beta, p_dtype, eps, None, stats, (xr.data, xr.scale))
-    return _matmul(xr, wr, dev, bias, 0, out_dtype), (xt.keep if want_xt else None), (wt.keep if want_wt else None)
+    return _matmul(x2, xr, wr, bias, out_dtype), (xt.keep if want_xt else None), (wt.keep if want_wt else None)
 
 
 def _linear_backward(g, dims, xt, wt, dtypes, want, grad_fmt):
@@ -258,12 +260,11 @@ def _linear_backward(g, dims, xt, wt, dtypes, want, grad_fmt):
     M, N, K = dims
     wx, ww, wb = want
     g2, ld = _matrix(g if g.dim() == 2 else g.reshape(M, N), "linear_fp8")
-    dev = g2.device
-    gr = _Held.new(M, N, grad_fmt, dev) if wx else None
-    gt = _Held.new(N, M, grad_fmt, dev) if ww or not wx else None
+    gr = _Held.new(M, N, grad_fmt, g2) if wx else None
+    gt = _Held.new(N, M, grad_fmt, g2) if ww or not wx else None
     db = _quantize(g2, ld, grad_fmt, gr, gt, colsum=wb)
-    dx = _matmul(gr, _Held.of(wt, K, N, 0), dev, None, 0, dtypes[0]) if wx else None
-    dw = _matmul(gt, _Held.of(xt, K, M, 0), dev, None, 0, dtypes[1]) if ww else None
+    dx = _matmul(g2, gr, _Held.of(wt, K, N, 0), None, dtypes[0]) if wx else None
+    dw = _matmul(g2, gt, _Held.of(xt, K, M, 0), None, dtypes[1]) if ww else None
     return dx, dw, db.to(dtypes[2]) if wb else None
 
 
@@ -339,7 +340,7 @@ class LayerNormLinearFp8(Function):
             ctx.save_for_backward()
             return x.new_empty((*x.shape[:-1], N))
         before = nx or ng or nbt                       # something in front of the product wants a gradient
-        stats = torch.empty((2, M), dtype=torch.float32, device=x.device) if before or nw else None
+        stats = x.new_empty((2, M), dtype=torch.float32) if before or nw else None
         y, xt, wt = _linear_forward(ctx, x2, ld, weight, bias, x.dtype, before, nw, what, (stats, gamma, beta, p_dtype, eps))
         ctx.save_for_backward(xt, wt, *((x2, stats, gamma) if before else (None, None, None)))
         return y if x2 is x else y.view(*x.shape[:-1], N)

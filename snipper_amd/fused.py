@@ -387,14 +387,13 @@ def ln_fusable(x: torch.Tensor, norm: torch.nn.LayerNorm) -> bool:
 _ROW_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 3}      # include/snipper_fp8.h
 
 
-def _call(fn, device, *args) -> None:
-    """fn(current stream of ``device``, *args) with that device current; raises on an error code."""
-    index = device.index
+def _call(fn, index: int, *args) -> None:
+    """fn(current stream of device ``index``, *args) with that device current; raises on an error code."""
     if index == torch._C._cuda_getDevice():
         rc = fn(torch._C._cuda_getCurrentRawStream(index), *args)
     else:
-        with torch.cuda.device(device):
-            rc = fn(_stream(device), *args)
+        with torch.cuda.device(index):
+            rc = fn(torch._C._cuda_getCurrentRawStream(index), *args)
     if rc:
         _lib.check(rc, fn.__name__)
 
@@ -450,26 +449,25 @@ def _layer_norm_forward(x2, ld, gamma, beta, p_dtype, eps, y, stats, blocks=(Non
     if R == 0:
         return
     mean = stats.data_ptr() if stats is not None else None
-    _call(_lib.load().snipper_layernorm_forward, x2.device, x2.data_ptr(), _ROW_DT[x2.dtype], ld, _opt(gamma), _opt(beta), _ROW_DT[p_dtype],
+    _call(_lib.load().snipper_layernorm_forward, x2.get_device(), x2.data_ptr(), _ROW_DT[x2.dtype], ld, _opt(gamma), _opt(beta), _ROW_DT[p_dtype],
           R, C, eps, _opt(y), mean, mean + 4 * R if mean is not None else None, blocks[0], blocks[1], fmt)
 
 
 def _layer_norm_backward(g, x2, ld, stats, gamma, p_dtype, want_dx, want_params):
     """(dx [rows, C], dgamma, dbeta) from g, contiguous and of x2's type; None for what is not wanted."""
     R, C = x2.shape
-    dev = x2.device
-    dx = torch.empty((R, C), dtype=x2.dtype, device=dev) if want_dx else None
+    dx = x2.new_empty((R, C)) if want_dx else None
     if not want_params and (R == 0 or not want_dx):
         return dx, None, None
     lib = _lib.load()
     dgamma = dbeta = ws = None
     nbytes = 0
     if want_params:
-        dgamma, dbeta = torch.empty(C, dtype=p_dtype, device=dev), torch.empty(C, dtype=p_dtype, device=dev)
+        dgamma, dbeta = x2.new_empty(C, dtype=p_dtype), x2.new_empty(C, dtype=p_dtype)
         nbytes = lib.snipper_layernorm_backward_workspace_bytes(R, C)
-        ws = torch.empty(nbytes // 4, dtype=torch.float32, device=dev) if nbytes else None
+        ws = stats.new_empty(nbytes // 4) if nbytes else None
     mean = stats.data_ptr()
-    _call(lib.snipper_layernorm_backward, dev, g.data_ptr(), x2.data_ptr(), _ROW_DT[x2.dtype], ld, mean, mean + 4 * R, _opt(gamma),
+    _call(lib.snipper_layernorm_backward, x2.get_device(), g.data_ptr(), x2.data_ptr(), _ROW_DT[x2.dtype], ld, mean, mean + 4 * R, _opt(gamma),
           _ROW_DT[p_dtype], R, C, _opt(dx), _opt(dgamma), _opt(dbeta), _opt(ws), nbytes)
     return dx, dgamma, dbeta
 
@@ -480,8 +478,8 @@ class LayerNormRows(Function):
     @staticmethod
     def forward(ctx, x, gamma, beta, normalized_shape, eps):
         x2, ld, p_dtype = _norm_rows(x, gamma, beta, normalized_shape, "layer_norm")
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        stats = torch.empty((2, x2.shape[0]), dtype=torch.float32, device=x.device)
+        y = x.new_empty(x.shape)
+        stats = x.new_empty((2, x2.shape[0]), dtype=torch.float32)
         _layer_norm_forward(x2, ld, gamma, beta, p_dtype, eps, y, stats)
         ctx.meta = p_dtype, ld, x.shape
         ctx.save_for_backward(x2, stats, gamma)
@@ -508,7 +506,7 @@ def layer_norm(x: torch.Tensor, norm: torch.nn.LayerNorm) -> torch.Tensor:
     if torch.is_grad_enabled() and (x.requires_grad or (gamma is not None and gamma.requires_grad) or (beta is not None and beta.requires_grad)):
         return LayerNormRows.apply(x, gamma, beta, norm.normalized_shape, norm.eps)
     x2, ld, p_dtype = _norm_rows(x, gamma, beta, norm.normalized_shape, "layer_norm")
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape)
     _layer_norm_forward(x2, ld, gamma, beta, p_dtype, norm.eps, y, None)
     return y
 

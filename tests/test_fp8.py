@@ -91,7 +91,7 @@ def test_c_quantize_refuses():
     assert call(x=None) == NULL and call(d=None) == NULL and call(s=None) == NULL and call(dt_=P) == NULL and call(mean=P) == NULL
     for bad in (dict(rows=0), dict(cols=0), dict(rows=(1 << 23) + 1), dict(cols=(1 << 23) + 1, ld=1 << 24), dict(ld=199), dict(dt=2), dict(dt=7),
                 dict(tile=64), dict(fmt=2), dict(pdt=2), dict(gamma=P), dict(d=ctypes.c_void_p(4104)), dict(s=ctypes.c_void_p(4098)),
-                dict(cs=P), dict(cs=P, ws=P, nb=4 * 200 - 1)):
+                dict(cs=P), dict(cs=P, ws=P, nb=4 * 200 - 1), dict(tile=128, mean=P, rstd=P)):
         assert call(**bad) == SHAPE, bad
     assert _lib.load().snipper_fp8_quantize_workspace_bytes(129, 200, 1) == 2 * 200 * 4
     assert _lib.load().snipper_fp8_quantize_workspace_bytes(129, 200, 0) == 0
@@ -105,7 +105,7 @@ def test_c_matmul_refuses():
     for n in ("a", "sa", "b", "sb", "out"):
         assert call(**{n: None}) == NULL, n
     for bad in (dict(M=0), dict(N=0), dict(K=0), dict(K=(1 << 23) + 1), dict(fa=2), dict(fb=-1), dict(odt=2), dict(bdt=2),
-                dict(a=ctypes.c_void_p(4104)), dict(sb=ctypes.c_void_p(4098))):
+                dict(a=ctypes.c_void_p(4104)), dict(sb=ctypes.c_void_p(4098)), dict(out=ctypes.c_void_p(4104))):
         assert call(**bad) == SHAPE, bad
     assert call(M=1 << 23, N=1 << 17) == SHAPE                                # (2^40 elements of a result)
     need = lib.snipper_fp8_matmul_workspace_bytes(384, 1024, 79000, 0)         # (a weight gradient: the reduction is split)

@@ -305,7 +305,7 @@ def _norm64(x, norm):
 
 @pytest.mark.parametrize("dtype", [E4M3, E5M2])
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 100), (17, 128), (5, 129), (9, 512), (4, 600), (3, 1100), (2, 2049), (2, 4097), (2, 8193), (2, 16384)])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 100), (17, 128), (5, 129), (33, 256), (18, 300), (9, 512), (4, 600), (3, 1100), (2, 2049), (2, 4097), (3, 8192), (2, 8193), (2, 16384)])
 def test_layer_norm_fp8(rows, cols, kind, dtype):
     x, norm = _x(rows, cols, DT[kind], spread=0.5), _norm(cols)
     with torch.no_grad():

@@ -61,7 +61,7 @@ def _run(x, g, norm):
     return [y.detach(), grads[0]] + [grads[1] if norm.weight is not None else None, grads[2] if norm.bias is not None else None]
 
 
-WIDTHS = [1, 2, 7, 127, 128, 129, 384, 511, 512, 513, 1024, 1027, 2048, 2050, 4096, 4099, 8192, 8200, 16383, 16384]
+WIDTHS = [1, 2, 7, 127, 128, 129, 256, 257, 383, 384, 385, 511, 512, 513, 1024, 1027, 2048, 2050, 4096, 4099, 8192, 8200, 16383, 16384]
 
 
 @pytest.mark.parametrize("kind,param", [("f32", "f32"), ("bf16", "f32"), ("bf16", "bf16"), ("f16", "f16"), ("f16", "f32")])
