@@ -35,12 +35,12 @@ extern "C" {
  * mean / rstd [rows] float32 (or both NULL): x is normalised first, (x - mean) * rstd * gamma + beta, gamma / beta [cols] of type
  * p_dtype or NULL (1 / 0); with tile_rows = 1 only.
  * Data pointers 16-byte, scale pointers 4-byte aligned.
- * colsum [cols] float32 or NULL: the sums of x over the rows, unrounded; needs snipper_fp8_quantize_workspace_bytes of workspace
- * (0 without it).  rows, cols <= 2^23. */
+ * colsum [cols] of type colsum_dtype or NULL: the sums of x over the rows, of the unrounded elements, in float32 and a fixed order;
+ * needs snipper_fp8_quantize_workspace_bytes of workspace (0 without it), 4-byte aligned.  rows, cols <= 2^23. */
 size_t snipper_fp8_quantize_workspace_bytes(int rows, int cols, int with_colsum);
 int snipper_fp8_quantize(void *stream, const void *x, int x_dtype, long long ldx, int rows, int cols, int tile_rows, int fmt,
                          const float *mean, const float *rstd, const void *gamma, const void *beta, int p_dtype,
-                         uint8_t *data, uint8_t *scale, uint8_t *data_t, uint8_t *scale_t, float *colsum,
+                         uint8_t *data, uint8_t *scale, uint8_t *data_t, uint8_t *scale_t, void *colsum, int colsum_dtype,
                          void *workspace, size_t workspace_bytes);
 
 /* out [M][N] = act(A [M][K] . B [N][K]^T + bias [N]) of two matrices in blocks; act = ReLU if relu, bias of type bias_dtype or NULL.

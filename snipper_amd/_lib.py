@@ -19,7 +19,7 @@ _BWD_ARGS = [c_void_p] * 7 + [c_int] * 7 + [c_void_p] * 3      # stream, grad_ou
 EXPORTS = {
     # include/snipper_fp8.h
     "snipper_fp8_quantize_workspace_bytes": ([c_int] * 3, c_size_t),
-    "snipper_fp8_quantize": ([c_void_p, c_void_p, c_int, c_longlong] + [c_int] * 4 + [c_void_p] * 4 + [c_int] + [c_void_p] * 6 +
+    "snipper_fp8_quantize": ([c_void_p, c_void_p, c_int, c_longlong] + [c_int] * 4 + [c_void_p] * 4 + [c_int] + [c_void_p] * 5 + [c_int, c_void_p] +
                              [c_size_t], c_int),
     "snipper_fp8_matmul_workspace_bytes": ([c_int] * 4, c_size_t),
     "snipper_fp8_matmul": ([c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int,

@@ -130,9 +130,11 @@ size_t snipper_fp8_quantize_workspace_bytes(int rows, int cols, int with_colsum)
 
 int snipper_fp8_quantize(void *stream, const void *x, int x_dtype, long long ldx, int rows, int cols, int tile_rows, int fmt,
                          const float *mean, const float *rstd, const void *gamma, const void *beta, int p_dtype, uint8_t *data,
-                         uint8_t *scale, uint8_t *data_t, uint8_t *scale_t, float *colsum, void *workspace, size_t workspace_bytes) {
+                         uint8_t *scale, uint8_t *data_t, uint8_t *scale_t, void *colsum, int colsum_dtype, void *workspace,
+                         size_t workspace_bytes) {
   if (!x || (!data && !data_t) || (data && !scale) || (data_t && !scale_t) || ((mean == nullptr) != (rstd == nullptr))) return SNIPPER_E_NULL;
-  if (!dim_ok(rows) || !dim_ok(cols) || ldx < cols || !type_ok(x_dtype) || !type_ok(p_dtype) || !fmt_ok(fmt)) return SNIPPER_E_SHAPE;
+  if (!dim_ok(rows) || !dim_ok(cols) || ldx < cols || !type_ok(x_dtype) || !type_ok(p_dtype) || !type_ok(colsum_dtype) || !fmt_ok(fmt))
+    return SNIPPER_E_SHAPE;
   if (tile_rows != 1 && (tile_rows != 128 || mean)) return SNIPPER_E_SHAPE;
   if (!mean && (gamma || beta)) return SNIPPER_E_SHAPE;
   if (((uintptr_t)data | (uintptr_t)data_t) & 15 || ((uintptr_t)scale | (uintptr_t)scale_t) & 3) return SNIPPER_E_SHAPE;
@@ -158,7 +160,7 @@ int snipper_fp8_quantize(void *stream, const void *x, int x_dtype, long long ldx
       else hipLaunchKernelGGL((quant_tile_kernel<T, F, false, false>), grid, dim3(512), 0, st, a);
     });
   });
-  if (colsum) hipLaunchKernelGGL(colsum_parts_kernel, dim3(ceil_div(cols, 32)), dim3(1024), 0, st, (const float *)workspace, rb, cols, colsum);
+  if (colsum) hipLaunchKernelGGL(colsum_parts_kernel, dim3(ceil_div(cols, 32)), dim3(1024), 0, st, (const float *)workspace, rb, cols, colsum, colsum_dtype);
   return launch_status();
 }
 

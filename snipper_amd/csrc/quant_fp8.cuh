@@ -196,10 +196,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(NORM ? 5 : 
 }
 
 // out[c] = sum_b part[b][c]
-__global__ __launch_bounds__(1024) void colsum_parts_kernel(const float *part, int nparts, int C, float *out) {
+__global__ __launch_bounds__(1024) void colsum_parts_kernel(const float *part, int nparts, int C, void *out, int out_dt) {
   const int c = blockIdx.x * 32 + (threadIdx.x & 31);
   const float s = sum_parts(part, nparts, C, c);
-  if (threadIdx.x < 32 && c < C) out[c] = s;
+  if (threadIdx.x < 32 && c < C) store_param(out, out_dt, c, s);
 }
 
 }  // namespace rows

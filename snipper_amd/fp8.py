@@ -59,26 +59,17 @@ class Fp8Blocks:
         return (self.data.float().view(R, P // 128, 128) * s[:, :, None]).view(R, P)[:, :self.cols]
 
 
-class _Held:
-    """The same inside this file: pointers into one buffer (or into an Fp8Blocks' tensors), so that a training step makes few tensors."""
+# Inside this file a matrix in blocks is (address of its data, of its scales): several lie in one buffer, each from a multiple of 256 on.
+def _room(rows: int, cols: int) -> int:
+    return (rows * (-(-cols // 128) * 128 + -(-cols // 512) * 4) + 255) & -256
 
-    __slots__ = ("keep", "data", "scale", "rows", "cols", "fmt")
 
-    def __init__(self, keep, data, scale, rows, cols, fmt):
-        self.keep, self.data, self.scale, self.rows, self.cols, self.fmt = keep, data, scale, rows, cols, fmt
+def _at(address: int, rows: int, cols: int) -> Tuple[int, int]:
+    return address, address + rows * (-(-cols // 128) * 128)
 
-    @staticmethod
-    def new(rows: int, cols: int, fmt: int, like: torch.Tensor) -> "_Held":
-        return _Held.of(like.new_empty(rows * (-(-cols // 128) * 128 + -(-cols // 512) * 4), dtype=torch.uint8), rows, cols, fmt)
 
-    @staticmethod
-    def of(buf, rows: int, cols: int, fmt: int) -> "_Held":
-        p = buf.data_ptr()
-        return _Held(buf, p, p + rows * (-(-cols // 128) * 128), rows, cols, fmt)
-
-    @staticmethod
-    def view(b: Fp8Blocks) -> "_Held":
-        return _Held(b, b.data.data_ptr(), b.scale.data_ptr(), b.data.shape[0], b.cols, _FMT[b.data.dtype])
+def _parts(b: Fp8Blocks) -> Tuple[int, int]:
+    return b.data.data_ptr(), b.scale.data_ptr()
 
 
 def _new_blocks(rows: int, cols: int, dtype, device) -> Fp8Blocks:
@@ -119,25 +110,20 @@ def _no_graph(what: str, *tensors) -> None:
         raise RuntimeError(f"{what} is not differentiable: use linear_fp8 / layer_norm_linear_fp8, or call it under torch.no_grad()")
 
 
-def _quantize(x2, ld, fmt, a=None, b=None, tile=False, colsum=False, norm=None):
-    """x into a (blocks of x) and / or b (blocks of x^T); the sums over the rows if ``colsum``.  ``norm``: (stats [2, R], gamma, beta,
-    p_dtype)."""
+_NONE = (None, None)
+
+
+def _quantize(x2, ld, fmt, a=_NONE, b=_NONE, tile=1, norm=None, colsum=None, ws=None, ws_bytes=0):
+    """x into a (blocks of x) and / or b (blocks of x^T); the sums over the rows into ``colsum`` if given.  ``norm``: (stats [2, R],
+    gamma, beta, p_dtype)."""
     R, C = x2.shape
-    lib = _lib.load()
-    s = ws = None
-    nbytes = 0
-    if colsum:
-        nbytes = lib.snipper_fp8_quantize_workspace_bytes(R, C, 1)
-        s, ws = x2.new_empty(C, dtype=torch.float32), x2.new_empty(nbytes // 4, dtype=torch.float32)
     mean = rstd = gamma = beta = None
     p_dtype = 0
     if norm is not None:
         mean, gamma, beta, p_dtype = norm[0].data_ptr(), _opt(norm[1]), _opt(norm[2]), _ROW_DT[norm[3]]
         rstd = mean + 4 * R
-    _call(lib.snipper_fp8_quantize, x2.get_device(), x2.data_ptr(), _ROW_DT[x2.dtype], ld, R, C, 128 if tile else 1, fmt, mean, rstd, gamma, beta, p_dtype,
-          a.data if a is not None else None, a.scale if a is not None else None, b.data if b is not None else None,
-          b.scale if b is not None else None, _opt(s), _opt(ws), nbytes)
-    return s
+    _call(_lib.load().snipper_fp8_quantize, x2.get_device(), x2.data_ptr(), _ROW_DT[x2.dtype], ld, R, C, tile, fmt, mean, rstd, gamma, beta, p_dtype,
+          a[0], a[1], b[0], b[1], _opt(colsum), _ROW_DT[colsum.dtype] if colsum is not None else 0, ws, ws_bytes)
 
 
 def quantize_rows(x: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> Fp8Blocks:
@@ -147,7 +133,7 @@ def quantize_rows(x: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> 
     x2, ld = _matrix(x, "quantize_rows")
     a = _new_blocks(*x2.shape, dtype, x.device)
     if x2.shape[0]:
-        _quantize(x2, ld, fmt, _Held.view(a))
+        _quantize(x2, ld, fmt, _parts(a))
     return a
 
 
@@ -159,7 +145,7 @@ def quantize_both(x: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> 
     if x2.shape[0] == 0:
         raise ValueError("quantize_both: a matrix without rows has no columns to cut into blocks")
     a, b = _new_blocks(*x2.shape, dtype, x.device), _new_blocks(x2.shape[1], x2.shape[0], dtype, x.device)
-    _quantize(x2, ld, fmt, _Held.view(a), _Held.view(b))
+    _quantize(x2, ld, fmt, _parts(a), _parts(b))
     return a, b
 
 
@@ -171,16 +157,12 @@ def quantize_tiles(w: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn) ->
         raise ValueError(f"quantize_tiles: a matrix with rows, got {tuple(w.shape)}")
     w2, ld = _matrix(w, "quantize_tiles")
     a, b = _new_blocks(*w2.shape, dtype, w.device), _new_blocks(w2.shape[1], w2.shape[0], dtype, w.device)
-    _quantize(w2, ld, fmt, _Held.view(a), _Held.view(b), tile=True)
+    _quantize(w2, ld, fmt, _parts(a), _parts(b), tile=128)
     return a, b
 
 
-def _matmul(like: torch.Tensor, a: _Held, b: _Held, bias, out_dtype):
-    return _product(like, a.data, a.scale, a.fmt, b.data, b.scale, b.fmt, a.rows, b.rows, a.cols, bias, 0, out_dtype)
-
-
-def _product(like, a_data, a_scale, a_fmt, b_data, b_scale, b_fmt, M, N, K, bias, relu, out_dtype):
-    """[M, N] on the device of ``like``."""
+def _product(like, a, a_fmt, b, b_fmt, M, N, K, bias, relu, out_dtype):
+    """act(a b^T + bias) [M, N] on the device of ``like``."""
     out = like.new_empty((M, N), dtype=out_dtype)
     if M == 0 or N == 0:
         return out
@@ -188,7 +170,7 @@ def _product(like, a_data, a_scale, a_fmt, b_data, b_scale, b_fmt, M, N, K, bias
     od = _ROW_DT[out_dtype]
     nbytes = lib.snipper_fp8_matmul_workspace_bytes(M, N, K, od)
     ws = like.new_empty(nbytes // 4, dtype=torch.float32) if nbytes else None
-    _call(lib.snipper_fp8_matmul, like.get_device(), a_data, a_scale, a_fmt, b_data, b_scale, b_fmt, M, N, K, _opt(bias),
+    _call(lib.snipper_fp8_matmul, like.get_device(), a[0], a[1], a_fmt, b[0], b[1], b_fmt, M, N, K, _opt(bias),
           _ROW_DT[bias.dtype] if bias is not None else 0, relu, out.data_ptr(), od, _opt(ws), nbytes)
     return out
 
@@ -219,8 +201,7 @@ def matmul_fp8(a: Fp8Blocks, b: Fp8Blocks, bias: Optional[torch.Tensor] = None, 
     if bias is not None:
         _no_graph("matmul_fp8", bias)
         _check_bias(bias, N, ad.device, "matmul_fp8")
-    return _product(ad, ad.data_ptr(), a.scale.data_ptr(), _FMT[ad.dtype], bd.data_ptr(), b.scale.data_ptr(), _FMT[bd.dtype], M, N, K, bias,
-                    int(relu), out_dtype)
+    return _product(ad, _parts(a), _FMT[ad.dtype], _parts(b), _FMT[bd.dtype], M, N, K, bias, int(relu), out_dtype)
 
 
 def _linear_params(x, weight, bias, what):
@@ -232,17 +213,20 @@ def _linear_params(x, weight, bias, what):
         _check_bias(bias, weight.shape[0], x.device, what)
 
 
-def _linear_forward(ctx, x2, ld, weight, bias, out_dtype, want_wt, want_xt, what, norm=None):
-    """y [M, N] of x2 [M, K] (normalised first with ``norm``); keeps on ctx what the backward pass reads: the columns' blocks of the
-    input (for dW) and of the weight (for dx)."""
+def _linear_forward(x2, ld, weight, bias, out_dtype, want_wt, want_xt, what, norm=None):
+    """y [M, N] of x2 [M, K] (normalised first with ``norm``), and a buffer of what the backward pass reads: the columns' blocks of the
+    input (for dW; in front) and of the weight (for dx)."""
     w2, ldw = _matrix(weight, what)
     M, K = x2.shape
     N = w2.shape[0]
-    wr = _Held.new(N, K, 0, x2)
-    wt = _Held.new(K, N, 0, x2) if want_wt else None
-    _quantize(w2, ldw, 0, wr, wt, tile=True)
-    xr = _Held.new(M, K, 0, x2)
-    xt = _Held.new(K, M, 0, x2) if want_xt else None
+    x_room = _room(M, K)
+    xt_room = _room(K, M) if want_xt else 0
+    rows = x2.new_empty(x_room + _room(N, K), dtype=torch.uint8)
+    keep = x2.new_empty(xt_room + (_room(K, N) if want_wt else 0), dtype=torch.uint8) if want_xt or want_wt else None
+    p = rows.data_ptr()
+    xr, wr = _at(p, M, K), _at(p + x_room, N, K)
+    _quantize(w2, ldw, 0, wr, _at(keep.data_ptr() + xt_room, K, N) if want_wt else _NONE, tile=128)
+    xt = _at(keep.data_ptr(), K, M) if want_xt else _NONE
     if norm is None:
         _quantize(x2, ld, 0, xr, xt)
     else:
@@ -251,21 +235,27 @@ def _linear_forward(ctx, x2, ld, weight, bias, out_dtype, want_wt, want_xt, what
             _layer_norm_forward(x2, ld, gamma, beta, p_dtype, eps, None, stats)
             _quantize(x2, ld, 0, xr, xt, norm=(stats, gamma, beta, p_dtype))
         else:
-            _layer_norm_forward(x2, ld, gamma, beta, p_dtype, eps, None, stats, (xr.data, xr.scale))
-    return _matmul(x2, xr, wr, bias, out_dtype), (xt.keep if want_xt else None), (wt.keep if want_wt else None)
+            _layer_norm_forward(x2, ld, gamma, beta, p_dtype, eps, None, stats, xr)
+    return _product(x2, xr, 0, wr, 0, M, N, K, bias, 0, out_dtype), keep
 
 
-def _linear_backward(g, dims, xt, wt, dtypes, want, grad_fmt):
-    """(dx [M, K] or None, dW or None, db or None) from the gradient [..., N]; dims (M, N, K); want = which; dtypes of the three."""
+def _linear_backward(g, dims, keep, dtypes, want, grad_fmt):
+    """(dx [M, K] or None, dW or None, db or None) from the gradient [..., N]; dims (M, N, K); dtypes of the three; want = which, the
+    first two as in the forward pass."""
     M, N, K = dims
     wx, ww, wb = want
     g2, ld = _matrix(g if g.dim() == 2 else g.reshape(M, N), "linear_fp8")
-    gr = _Held.new(M, N, grad_fmt, g2) if wx else None
-    gt = _Held.new(N, M, grad_fmt, g2) if ww or not wx else None
-    db = _quantize(g2, ld, grad_fmt, gr, gt, colsum=wb)
-    dx = _matmul(g2, gr, _Held.of(wt, K, N, 0), None, dtypes[0]) if wx else None
-    dw = _matmul(g2, gt, _Held.of(xt, K, M, 0), None, dtypes[1]) if ww else None
-    return dx, dw, db.to(dtypes[2]) if wb else None
+    ws_bytes = _lib.load().snipper_fp8_quantize_workspace_bytes(M, N, 1) if wb else 0
+    g_room, t_room = _room(M, N) if wx else 0, _room(N, M) if ww or not wx else 0
+    buf = g2.new_empty(g_room + t_room + ws_bytes, dtype=torch.uint8)
+    p = buf.data_ptr()
+    gr, gt = _at(p, M, N) if wx else _NONE, _at(p + g_room, N, M) if t_room else _NONE
+    db = g2.new_empty(N, dtype=dtypes[2]) if wb else None
+    _quantize(g2, ld, grad_fmt, gr, gt, colsum=db, ws=p + g_room + t_room if wb else None, ws_bytes=ws_bytes)
+    k = keep.data_ptr() if keep is not None else 0
+    dx = _product(g2, gr, grad_fmt, _at(k + (_room(K, M) if ww else 0), K, N), 0, M, K, N, None, 0, dtypes[0]) if wx else None
+    dw = _product(g2, gt, grad_fmt, _at(k, K, M), 0, N, K, M, None, 0, dtypes[1]) if ww else None
+    return dx, dw, db
 
 
 def _zero_grads(g, shapes, dtypes, want):
@@ -284,8 +274,8 @@ class LinearFp8(Function):
         if M == 0:
             ctx.save_for_backward()
             return x.new_empty((*x.shape[:-1], N))
-        y, xt, wt = _linear_forward(ctx, x2, ld, weight, bias, x.dtype, ctx.needs_input_grad[0], ctx.needs_input_grad[1], "linear_fp8")
-        ctx.save_for_backward(xt, wt)
+        y, keep = _linear_forward(x2, ld, weight, bias, x.dtype, ctx.needs_input_grad[0], ctx.needs_input_grad[1], "linear_fp8")
+        ctx.save_for_backward(keep)
         return y if x2 is x else y.view(*x.shape[:-1], N)
 
     @staticmethod
@@ -295,8 +285,8 @@ class LinearFp8(Function):
         want = ctx.needs_input_grad[:3]
         if dims[0] == 0:
             return *_zero_grads(g, (shape, dims[1:], dims[1]), dtypes, want), None
-        xt, wt = ctx.saved_tensors
-        dx, dw, db = _linear_backward(g, dims, xt, wt, dtypes, want, grad_fmt)
+        keep, = ctx.saved_tensors
+        dx, dw, db = _linear_backward(g, dims, keep, dtypes, want, grad_fmt)
         return dx.view(shape) if dx is not None and len(shape) != 2 else dx, dw, db, None
 
 
@@ -341,8 +331,8 @@ class LayerNormLinearFp8(Function):
             return x.new_empty((*x.shape[:-1], N))
         before = nx or ng or nbt                       # something in front of the product wants a gradient
         stats = x.new_empty((2, M), dtype=torch.float32) if before or nw else None
-        y, xt, wt = _linear_forward(ctx, x2, ld, weight, bias, x.dtype, before, nw, what, (stats, gamma, beta, p_dtype, eps))
-        ctx.save_for_backward(xt, wt, *((x2, stats, gamma) if before else (None, None, None)))
+        y, keep = _linear_forward(x2, ld, weight, bias, x.dtype, before, nw, what, (stats, gamma, beta, p_dtype, eps))
+        ctx.save_for_backward(keep, *((x2, stats, gamma) if before else (None, None, None)))
         return y if x2 is x else y.view(*x.shape[:-1], N)
 
     @staticmethod
@@ -354,9 +344,9 @@ class LayerNormLinearFp8(Function):
         if M == 0:
             return *_zero_grads(g, (shape, K, K, (N, K), N), dtypes, want), None, None, None
         nx, ng, nbt, nw, nb = want
-        xt, wt, x2, stats, gamma = ctx.saved_tensors
+        keep, x2, stats, gamma = ctx.saved_tensors
         before = nx or ng or nbt
-        dz, dw, db = _linear_backward(g, dims, xt, wt, (dtypes[0], dtypes[3], dtypes[4]), (before, nw, nb), grad_fmt)
+        dz, dw, db = _linear_backward(g, dims, keep, (dtypes[0], dtypes[3], dtypes[4]), (before, nw, nb), grad_fmt)
         dx = dgamma = dbeta = None
         if before:
             dx, dgamma, dbeta = _layer_norm_backward(dz, x2, ld, stats, gamma, dtypes[1], nx, ng or nbt)

@@ -86,12 +86,12 @@ def test_c_quantize_refuses():
     f = _lib.load().snipper_fp8_quantize
 
     def call(x=P, dt=0, ld=200, rows=4, cols=200, tile=1, fmt=0, mean=None, rstd=None, gamma=None, beta=None, pdt=0, d=P, s=P, dt_=None,
-             st_=None, cs=None, ws=None, nb=0):
-        return f(None, x, dt, ld, rows, cols, tile, fmt, mean, rstd, gamma, beta, pdt, d, s, dt_, st_, cs, ws, nb)
+             st_=None, cs=None, cdt=0, ws=None, nb=0):
+        return f(None, x, dt, ld, rows, cols, tile, fmt, mean, rstd, gamma, beta, pdt, d, s, dt_, st_, cs, cdt, ws, nb)
     assert call(x=None) == NULL and call(d=None) == NULL and call(s=None) == NULL and call(dt_=P) == NULL and call(mean=P) == NULL
     for bad in (dict(rows=0), dict(cols=0), dict(rows=(1 << 23) + 1), dict(cols=(1 << 23) + 1, ld=1 << 24), dict(ld=199), dict(dt=2), dict(dt=7),
                 dict(tile=64), dict(fmt=2), dict(pdt=2), dict(gamma=P), dict(d=ctypes.c_void_p(4104)), dict(s=ctypes.c_void_p(4098)),
-                dict(cs=P), dict(cs=P, ws=P, nb=4 * 200 - 1), dict(tile=128, mean=P, rstd=P)):
+                dict(cs=P), dict(cs=P, cdt=2, ws=P, nb=4 * 200), dict(cs=P, ws=P, nb=4 * 200 - 1), dict(tile=128, mean=P, rstd=P)):
         assert call(**bad) == SHAPE, bad
     assert _lib.load().snipper_fp8_quantize_workspace_bytes(129, 200, 1) == 2 * 200 * 4
     assert _lib.load().snipper_fp8_quantize_workspace_bytes(129, 200, 0) == 0
