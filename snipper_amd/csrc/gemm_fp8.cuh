@@ -155,8 +155,13 @@ __device__ __forceinline__ void each_step(F &&f, std::integer_sequence<int, K...
 // Rows go to LDS by DMA in 16-byte pieces, piece c of row r at place c ^ key(r), and a lane takes pieces g and g + 4 of its row (both
 // sides alike), so that reads are free of bank conflicts: a 16-byte read serves lanes 0-3, 12-15, 20-27, then 4-11, 16-19, 28-31, then
 // the same of the upper half, 256 bytes each (counted; keys that suit groups of 8 or 16 neighbours cost twice the clocks).  A:
-// consecutive rows, key = r & 7; B: rows of mm_pair_row, key = bits 0, 1 and 3 of r; two buffers, one barrier a step.  The scale words of four K steps come the same way (plain loads of them would make
-// the compiler wait for the DMAs issued after them).
+// consecutive rows, key = r & 7; B: rows of mm_pair_row, key = bits 0, 1 and 3 of r; two buffers, one barrier a step.  The scale words
+// of four K steps come the same way (plain loads of them would make the compiler wait for the DMAs issued after them).
+// 8192^3 in tiles of 256 x 256 by eight waves of 128 x 64: 458 us, 2.4 PFLOP/s, where the instructions alone reach 3.65 .. 4.45 on such
+// data and a large library product 2.98.  A K step takes 64 KB from the L2 into LDS for 33.5 MFLOP a CU, and the LDS reads of its waves
+// and that fill share the LDS; four waves of 128 x 128, which read less, hold half the rows in flight (510 .. 568 us), operands
+// straight from the L2 735, steps of half a block with the 32 x 32 x 64 instruction 558, touching lines a step ahead 491.  EXACT: 79 000
+// x 1024 x 384's weight gradient 72 us = 0.86 PFLOP/s; the bfloat16 instructions' own limit is 43 us, the rest is widening.
 // INWARD (M >= BM, N >= BN): the last tile of an edge is moved inwards, and two workgroups store the same values; rows need no range
 // checks then, and their addresses one register a side instead of one for each load.
 template <int FA, int FB, bool EXACT, int WM, int WN, int TM, int TN, bool INWARD>
@@ -327,7 +332,8 @@ __device__ __forceinline__ void issue_chunk(const MmArgs &a, unsigned char *slot
 // chunks.  A tile kernel of such shapes spends its time filling and draining: its two or three K steps do not cover the latency of
 // their loads, nor the stores of the tile before.  Here loads run S - 1 chunks ahead across the stores; the counted waits rely on every
 // wave issuing the same number of memory instructions per chunk, so rows and columns past the end go through the buffers' range
-// checks.  The workgroups that share a chunk sit on one XCD: A comes from HBM once.  Results go past the caches: 79 000 x 1024 x 384 54 -> 49 us.
+// checks.  The workgroups that share a chunk sit on one XCD: A comes from HBM once.  Results go past the caches: 79 000 x 1024 x 384
+// 54 -> 49 us (tiles of 128 x 128: 100), 193 MB at 3.9 TB/s, nearly all of them stores.
 template <int FA, int FB, int KS>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void mm_stationary_kernel(MmArgs a, int n_series) {
   constexpr int ROWS = 64, PB = KS * 128, S = KS <= 4 ? 4 : KS <= 6 ? 3 : 2, QW = (KS + 3) / 4, kChunk = ROWS * PB, kScl = ROWS * QW * 4;
@@ -427,7 +433,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // ---- few rows -----------------------------------------------------------------------------------------------------------
 // At most 16 rows of A: B's bytes count, and they are read once, straight into registers.  A workgroup of W waves makes 16 columns; the
 // waves take every W-th group of four K steps (a word of scales; all of a group's loads are on the way before its first product) and
-// add their sums through LDS in a fixed order.
+// add their sums through LDS in a fixed order.  Bound by latency and HBM: 1 x 4096 x 4096 6.6 us (17 MB, 2.5 TB/s), 1 x 8192 x 8192 15 us
+// (67 MB, 4.5 TB/s).
 template <int FA, int FB, bool EXACT>
 __global__ __launch_bounds__(512) void mm_rows_kernel(MmArgs a) {
   __shared__ f32x4 red[8][64];
