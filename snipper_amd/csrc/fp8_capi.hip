@@ -96,6 +96,7 @@ MmPlan mm_plan(int M, int N, int K, bool exact) {
   }
   // The largest tile that still gives every CU one: 4096^3 66 (256) against 71 (128); 8192 x 1024 x 4096 38 (128) against 57 (256), 55
   // (64); 1024^3 6 (64) against 10 (128).  Few tiles and a long K axis: larger tiles, which load less, and more pieces
+  // (256 x 128 or 128 x 256 never won: 4096 x 1024 x 8192 61 against 48 of 128 x 128, 8192^3 513 .. 544 against 457 of 256 x 256)
   const long long t128 = (long long)ceil_div(M, 128) * ceil_div(N, 128);
   if (!exact && M >= 256 && N >= 256 && (long long)ceil_div(M, 256) * ceil_div(N, 256) >= kCUs) p.kind = 2;
   else p.kind = t128 >= kCUs || steps >= 64 ? 1 : 4;

@@ -11,8 +11,6 @@ typedef _Float16 f16_t;
 typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
 typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
 
-constexpr int kBlock = 128;                       // elements behind one scale
-
 enum { kF32 = 0, kBF16 = 1, kF16 = 3 };           // type codes of the C ABI
 
 // W consecutive elements of a row as float.  The address needs no more than the element's own alignment: memory instructions take any

@@ -16,6 +16,9 @@ Blocks run along the axis that a product sums over.  The training step therefore
 transpose holds the same values.  Scales are powers of two that keep the largest element of a block in range: nothing saturates, and
 an element is its input rounded once.  CUDA tensors only, as everywhere in this package; autocast changes nothing here, a result has
 x's type.
+
+Every call can be captured into a graph.  A captured backward pass needs what PyTorch asks of any: leaves whose eager graphs are gone
+(the engine would otherwise join the capture to the stream that those were made on).
 """
 from __future__ import annotations
 
