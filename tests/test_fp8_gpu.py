@@ -189,6 +189,52 @@ def test_matmul_beyond_32_bit_offsets():
         assert (y[:-100].double() - e).norm() <= (torch.finfo(out).eps / 2 + 2e-4) * e.norm() * (M - 100) ** 0.5
 
 
+def test_the_longest_rows():
+    """2^23 elements: few rows, pieces of tiles, and whole tiles whose rows end 2^31 bytes behind a tile's first."""
+    K = 1 << 23
+    for M, N in ((3, 5), (20, 40)):
+        a, b = (fp8.quantize_rows(torch.randn(n, K, device=DEV, dtype=torch.bfloat16)) for n in (M, N))
+        e = torch.zeros(M, N, dtype=torch.float64, device=DEV)
+        for at in range(0, K, 1 << 20):
+            A, B = (x.data[:, at:at + (1 << 20)].double() * x.scale.float().double()[:, at // 128:at // 128 + 8192].repeat_interleave(128, 1) for x in (a, b))
+            e += A @ B.t()
+        # up to 2^15 additions in turn, each off by 2^-24 of a partial sum at most: 2^-24 sqrt(2^15) = 1.1e-5 where they are independent,
+        # taken ten times; the 8-bit instructions' own 1.5e-5 twenty times; a block of 128 left out would be 2^-8
+        for out, most in ((torch.float32, 1.1e-4), (torch.bfloat16, 2.0 ** -9 + 3e-4)):
+            assert (fp8.matmul_fp8(a, b, out_dtype=out).double() - e).norm() <= most * e.norm()
+    M = 4096
+    bytes_ = [torch.zeros(M, K, dtype=torch.uint8, device=DEV) for _ in range(2)]
+    scale = torch.full((M, K // 128), 127, dtype=torch.uint8, device=DEV).view(torch.float8_e8m0fnu)
+    one, two = 0x38, 0x40                                                          # (1 and 2 in e4m3)
+    for row, at in ((0, 0), (255, K - 1), (4095, K - 1), (3841, K // 2)):
+        bytes_[0][row, at], bytes_[1][row, at] = one, two
+    y = fp8.matmul_fp8(*(fp8.Fp8Blocks(d.view(E4M3), scale, K) for d in bytes_))
+    e = torch.zeros(M, M, device=DEV, dtype=torch.bfloat16)
+    for r, c in ((0, 0), (255, 255), (4095, 4095), (255, 4095), (4095, 255), (3841, 3841)):
+        e[r, c] = 2
+    assert torch.equal(y, e)
+
+
+def test_more_than_four_million_rows():
+    """The quantizers' third grid axis, and results whose last rows lie more than 2^32 bytes behind the first."""
+    rows, K, N = (1 << 22) + 300, 70, 520
+    x = torch.randn(rows, K, device=DEV, dtype=torch.bfloat16)
+    a, at = fp8.quantize_both(x)
+    ta, tat = fp8.quantize_both(x[-300:])                                         # (2^22 is a multiple of 128: the same blocks)
+    u8 = lambda t: t.view(torch.uint8)
+    assert torch.equal(u8(a.data)[-300:], u8(ta.data)) and torch.equal(u8(a.scale)[-300:], u8(ta.scale))
+    assert torch.equal(u8(at.data)[:, 1 << 22:], u8(tat.data)) and torch.equal(u8(at.scale)[:, 1 << 15:(1 << 15) + 3], u8(tat.scale)[:, :3])
+    r = fp8.quantize_rows(x)
+    assert torch.equal(u8(r.data), u8(a.data)) and torch.equal(u8(r.scale), u8(a.scale))
+    assert torch.equal(at.dequantize()[:, :1000], fp8.quantize_both(x[:1024])[1].dequantize()[:, :1000])
+    w = fp8.quantize_rows(torch.randn(N, K, generator=_gen(4)).to(DEV))
+    bias = torch.randn(N, generator=_gen(5)).to(DEV)
+    for out in (torch.bfloat16, torch.float32):
+        y = fp8.matmul_fp8(a, w, bias, out_dtype=out)
+        _check_product(y[-300:], ta, w, bias, False, out)
+        _check_product(y[:300], fp8.quantize_rows(x[:300]), w, bias, False, out)
+
+
 # ---- training ----------------------------------------------------------------------------------------------------------
 def _linear(n, k, dtype, bias=True, seed=5):
     lin = torch.nn.Linear(k, n, bias=bias)

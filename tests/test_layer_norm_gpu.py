@@ -184,6 +184,28 @@ def test_against_differences():
         assert (want - got).abs() <= 2 * h * h * scale + 8440 ** 0.5 * 2 ** -22 / h * g.abs().max().double()
 
 
+@pytest.mark.parametrize("cols", [300, 600])
+def test_rows_beyond_32_bit_offsets(cols):
+    """Two and a half (five) GB in bfloat16: the last rows' results are those of the same rows alone."""
+    rows, last = (1 << 22) + 77, 77
+    x = torch.randn(rows, cols, device=DEV, dtype=torch.bfloat16)
+    g = torch.zeros(rows, cols, device=DEV, dtype=torch.bfloat16)
+    g[-last:] = torch.randn(last, cols, device=DEV, dtype=torch.bfloat16)
+    norm = torch.nn.LayerNorm(cols, device=DEV)
+
+    def both(x, g):
+        x = x.clone().requires_grad_()
+        y = fused.layer_norm(x, norm)
+        return (y.detach(), *torch.autograd.grad(y, (x, norm.weight, norm.bias), g))
+    y, dx, dw, db = both(x, g)
+    ys, dxs, dws, dbs = both(x[-last:], g[-last:])
+    assert torch.equal(y[-last:], ys) and torch.equal(dx[-last:], dxs) and not dx[:-last].any()
+    # the same 77 summands (and zeros) in another order: each of fewer than 77 additions is off by half a step of a sum
+    h = torch.nn.functional.layer_norm(x[-last:].float(), (cols,))
+    for a, b, S in ((dw, dws, (g[-last:].float() * h).abs().sum(0)), (db, dbs, g[-last:].float().abs().sum(0))):
+        assert ((a - b).abs() <= 2 * 77 * 2.0 ** -24 * 1.01 * S).all()
+
+
 def test_same_result_every_time_and_in_graphs():
     x, norm = torch.randn(3000, 384, generator=_gen(1)).to(DEV).requires_grad_(), _norm(384, torch.float32)
     g = torch.randn(3000, 384, generator=_gen(2)).to(DEV)
