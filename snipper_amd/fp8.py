@@ -28,7 +28,7 @@ import torch
 
 from . import _lib
 from ._autograd import Function
-from .fused import _ROW_DT, _call, _layer_norm_backward, _layer_norm_forward, _norm_rows, _once_differentiable, _opt
+from .fused import _ROW_DT, _call, _layer_norm_backward, _layer_norm_forward, _norm_rows, _once_differentiable, _opt, _row_stride
 
 _FMT = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}
 _MAX_DIM = 1 << 23
@@ -94,12 +94,7 @@ def _matrix(x: torch.Tensor, what: str):
     R = x2.shape[0]
     if not 1 <= C <= _MAX_DIM or R > _MAX_DIM:
         raise ValueError(f"{what}: up to 2^23 rows of 1 to 2^23 elements, got {tuple(shape)}")
-    if R <= 1 and x2.stride(1) == 1:
-        return x2, C
-    ld, inner = x2.stride()
-    if inner != 1 or ld < C:
-        x2, ld = x2.contiguous(), C
-    return x2, ld
+    return _row_stride(x2)
 
 
 def _format(dtype, what: str) -> int:
@@ -255,6 +250,7 @@ def _linear_backward(g, dims, keep, dtypes, want, grad_fmt):
     gr, gt = _at(p, M, N) if wx else _NONE, _at(p + g_room, N, M) if t_room else _NONE
     db = g2.new_empty(N, dtype=dtypes[2]) if wb else None
     _quantize(g2, ld, grad_fmt, gr, gt, colsum=db, ws=p + g_room + t_room if wb else None, ws_bytes=ws_bytes)
+    keep = keep.contiguous() if keep is not None else None          # (saved-tensor hooks may have changed its stride)
     k = keep.data_ptr() if keep is not None else 0
     dx = _product(g2, gr, grad_fmt, _at(k + (_room(K, M) if ww else 0), K, N), 0, M, K, N, None, 0, dtypes[0]) if wx else None
     dw = _product(g2, gt, grad_fmt, _at(k, K, M), 0, N, K, M, None, 0, dtypes[1]) if ww else None
@@ -328,7 +324,7 @@ class LayerNormLinearFp8(Function):
         if M > _MAX_DIM:
             raise ValueError(f"{what}: up to 2^23 rows")
         nx, ng, nbt, nw, nb = ctx.needs_input_grad[:5]
-        ctx.meta = (M, N, K), (x.dtype, p_dtype, p_dtype, weight.dtype, bias.dtype if bias is not None else None), grad_fmt, x.shape, ld
+        ctx.meta = (M, N, K), (x.dtype, p_dtype, p_dtype, weight.dtype, bias.dtype if bias is not None else None), grad_fmt, x.shape
         if M == 0:
             ctx.save_for_backward()
             return x.new_empty((*x.shape[:-1], N))
@@ -341,7 +337,7 @@ class LayerNormLinearFp8(Function):
     @staticmethod
     @_once_differentiable
     def backward(ctx, g):
-        dims, dtypes, grad_fmt, shape, ld = ctx.meta
+        dims, dtypes, grad_fmt, shape = ctx.meta
         M, N, K = dims
         want = ctx.needs_input_grad[:5]
         if M == 0:
@@ -352,7 +348,7 @@ class LayerNormLinearFp8(Function):
         dz, dw, db = _linear_backward(g, dims, keep, (dtypes[0], dtypes[3], dtypes[4]), (before, nw, nb), grad_fmt)
         dx = dgamma = dbeta = None
         if before:
-            dx, dgamma, dbeta = _layer_norm_backward(dz, x2, ld, stats, gamma, dtypes[1], nx, ng or nbt)
+            dx, dgamma, dbeta = _layer_norm_backward(dz, x2, stats, gamma, dtypes[1], nx, ng or nbt)
         return (dx.view(shape) if nx and len(shape) != 2 else dx, dgamma if ng else None, dbeta if nbt else None, dw, db, None, None, None)
 
 

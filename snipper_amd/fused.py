@@ -411,6 +411,17 @@ def _opt(t):
     return t.data_ptr() if t is not None else None
 
 
+def _row_stride(x2: torch.Tensor):
+    """x2 [rows, C], copied unless it has unit stride inside a row and rows that do not overlap, and its row stride."""
+    R, C = x2.shape
+    ld, inner = x2.stride()
+    if R <= 1 and inner == 1:
+        return x2, C
+    if inner != 1 or ld < C:
+        return x2.contiguous(), C
+    return x2, ld
+
+
 def _norm_rows(x: torch.Tensor, gamma, beta, normalized_shape, what: str):
     """(x as [rows, C] with unit stride inside a row, row stride, parameter type) of a layer norm over x's last axis."""
     if not x.is_cuda:
@@ -432,15 +443,9 @@ def _norm_rows(x: torch.Tensor, gamma, beta, normalized_shape, what: str):
     if gamma is not None and beta is not None and gamma.dtype is not beta.dtype:
         raise TypeError(f"{what}: weight and bias of one type")
     x2 = x if len(shape) == 2 else x.reshape(-1, C)
-    R = x2.shape[0]
-    if R >= 2 ** 31:
+    if x2.shape[0] >= 2 ** 31:
         raise ValueError(f"{what}: fewer than 2^31 rows")
-    ld, inner = x2.stride()
-    if R <= 1 and inner == 1:
-        return x2, C, p_dtype
-    if inner != 1 or ld < C:
-        x2, ld = x2.contiguous(), C
-    return x2, ld, p_dtype
+    return *_row_stride(x2), p_dtype
 
 
 def _layer_norm_forward(x2, ld, gamma, beta, p_dtype, eps, y, stats, blocks=(None, None), fmt=0):
@@ -453,8 +458,12 @@ def _layer_norm_forward(x2, ld, gamma, beta, p_dtype, eps, y, stats, blocks=(Non
           R, C, eps, _opt(y), mean, mean + 4 * R if mean is not None else None, blocks[0], blocks[1], fmt)
 
 
-def _layer_norm_backward(g, x2, ld, stats, gamma, p_dtype, want_dx, want_params):
-    """(dx [rows, C], dgamma, dbeta) from g, contiguous and of x2's type; None for what is not wanted."""
+def _layer_norm_backward(g, x2, stats, gamma, p_dtype, want_dx, want_params):
+    """(dx [rows, C], dgamma, dbeta) from g, contiguous and of x2's type; None for what is not wanted.  x2, stats and gamma as the
+    graph gives them back: saved-tensor hooks (torch.autograd.graph.save_on_cpu among them) may have changed their strides."""
+    x2, ld = _row_stride(x2)
+    stats = stats.contiguous()
+    gamma = gamma.contiguous() if gamma is not None else None
     R, C = x2.shape
     dx = x2.new_empty((R, C)) if want_dx else None
     if not want_params and (R == 0 or not want_dx):
@@ -481,7 +490,7 @@ class LayerNormRows(Function):
         y = x.new_empty(x.shape)
         stats = x.new_empty((2, x2.shape[0]), dtype=torch.float32)
         _layer_norm_forward(x2, ld, gamma, beta, p_dtype, eps, y, stats)
-        ctx.meta = p_dtype, ld, x.shape
+        ctx.meta = p_dtype, x.shape
         ctx.save_for_backward(x2, stats, gamma)
         return y
 
@@ -489,11 +498,11 @@ class LayerNormRows(Function):
     @_once_differentiable
     def backward(ctx, g):
         x2, stats, gamma = ctx.saved_tensors
-        p_dtype, ld, shape = ctx.meta
+        p_dtype, shape = ctx.meta
         wx, wg, wb = ctx.needs_input_grad[:3]
         if g.dtype is not x2.dtype or not g.is_contiguous():
             g = g.to(x2.dtype).contiguous()
-        dx, dgamma, dbeta = _layer_norm_backward(g, x2, ld, stats, gamma, p_dtype, wx, wg or wb)
+        dx, dgamma, dbeta = _layer_norm_backward(g, x2, stats, gamma, p_dtype, wx, wg or wb)
         return dx.view(shape) if wx and len(shape) != 2 else dx, dgamma if wg else None, dbeta if wb else None, None, None
 
 

@@ -1,0 +1,82 @@
+"""What the 8-bit operators' and the wide layer norm's wrappers hand to the native entries, on the CPU: the calls are recorded, not made."""
+import pytest
+import torch
+
+from snipper_amd import _lib, fp8, fused
+
+
+class OnCard(torch.Tensor):
+    """A CPU tensor that says that it is on the card, and whose results do."""
+    is_cuda = True
+
+
+def _card(t):
+    return t.as_subclass(OnCard)
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """(entry's name, arguments without the stream) of each native call, in turn."""
+    made = []
+
+    def record(fn, index, *args):
+        made.append((fn.__name__, args))
+    _lib.load()
+    for module in (fused, fp8):
+        monkeypatch.setattr(module, "_call", record)
+    return made
+
+
+def _dense(t):
+    return t.detach().clone(memory_format=torch.contiguous_format)
+
+
+HOOKS = {"none": (lambda t: t, lambda t: t),
+         "dense": (_dense, lambda t: t),                                     # what torch.autograd.graph.save_on_cpu gives back
+         "columns": (lambda t: t, lambda t: _dense(t.t()).t() if t.dim() == 2 else torch.stack([t, t], 1)[:, 0]),
+         "wider": (lambda t: t, lambda t: torch.cat([t, t], -1)[..., :t.shape[-1]] if t.dim() == 2 else t)}
+
+
+def _layer_norm_backward_call(made):
+    (_, args), = [c for c in made if c[0] == "snipper_layernorm_backward"]
+    return dict(zip(("g", "x", "dtype", "ldx", "mean", "rstd", "gamma", "p_dtype", "rows", "cols"), args))
+
+
+@pytest.mark.parametrize("hook", HOOKS)
+@pytest.mark.parametrize("op", ["layer_norm", "layer_norm_linear_fp8"])
+def test_backward_steps_by_the_stride_of_the_rows_that_it_gets(op, hook, calls):
+    """Saved-tensor hooks may give x back in another layout: each row that the native call reads lies inside the tensor handed to it."""
+    rows, cols, held = 6, 40, []
+    pack, unpack = HOOKS[hook]
+
+    def keep(t):
+        t = unpack(t)
+        held.append(t)
+        return t
+    x = _card(torch.randn(rows, cols + 9)[:, :cols]).requires_grad_()
+    norm, lin = torch.nn.LayerNorm(cols), torch.nn.Linear(cols, 8)
+    for m in (norm, lin):
+        for n, p in list(m.named_parameters()):
+            setattr(m, n, torch.nn.Parameter(_card(p.detach()), requires_grad=True))
+    with torch.autograd.graph.saved_tensors_hooks(pack, keep):
+        y = fused.layer_norm(x, norm) if op == "layer_norm" else fp8.layer_norm_linear_fp8(x, norm, lin)
+        torch.autograd.grad(y, x, torch.ones_like(y))
+    c = _layer_norm_backward_call(calls)
+    assert (c["rows"], c["cols"]) == (rows, cols) and c["ldx"] >= cols
+    given = [t for t in held if t.data_ptr() == c["x"]]
+    # a copy made for the call is contiguous; anything else is one of the tensors that the hooks gave back
+    if given:
+        t, = given
+        assert t.stride() == (c["ldx"], 1)
+    else:
+        assert c["ldx"] == cols
+    last = c["x"] + 4 * ((rows - 1) * c["ldx"] + cols)
+    # the statistics and what the products read are vectors for the native calls
+    for t in held:
+        if t.data_ptr() in (c["mean"], c["gamma"]):
+            assert t.is_contiguous()
+    assert c["rstd"] == c["mean"] + 4 * rows
+    starts = {t.data_ptr(): t for t in held if not t.is_contiguous()}
+    assert not any(a in starts for name, args in calls if name == "snipper_fp8_matmul" for a in args)
+    for t in given:
+        assert last <= t.untyped_storage().data_ptr() + t.untyped_storage().nbytes()
