@@ -28,7 +28,8 @@ import torch
 
 from . import _lib
 from ._autograd import Function
-from .fused import _ROW_DT, _call, _layer_norm_backward, _layer_norm_forward, _norm_rows, _once_differentiable, _opt, _row_stride
+from .fused import (_ROW_DT, _call, _differentiates, _layer_norm_backward, _layer_norm_forward, _norm_rows, _once_differentiable, _opt,
+                    _row_stride)
 
 _FMT = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}
 _MAX_DIM = 1 << 23
@@ -104,8 +105,9 @@ def _format(dtype, what: str) -> int:
 
 
 def _no_graph(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} is not differentiable: use linear_fp8 / layer_norm_linear_fp8, or call it under torch.no_grad()")
+    if _differentiates(*tensors):
+        raise RuntimeError(f"{what} is not differentiable: use linear_fp8 / layer_norm_linear_fp8, or call it under torch.no_grad() "
+                           "(and, in forward mode, on tensors without a tangent)")
 
 
 _NONE = (None, None)

@@ -8,6 +8,7 @@ from typing import List, Optional, Sequence
 
 import torch
 from ._autograd import Function
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -407,6 +408,16 @@ def _once_differentiable(backward):
     return run
 
 
+def _has_tangent(*tensors) -> bool:
+    """Whether a forward-mode derivative would be lost: a dual tensor's requires_grad is false, and no_grad leaves that mode on."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def _differentiates(*tensors) -> bool:
+    """Whether a call on these tensors goes through its autograd function (which refuses forward mode)."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or _has_tangent(*tensors)
+
+
 def _opt(t):
     return t.data_ptr() if t is not None else None
 
@@ -512,7 +523,7 @@ def layer_norm(x: torch.Tensor, norm: torch.nn.LayerNorm) -> torch.Tensor:
     bias.  The result and dx have x's type, dgamma and dbeta the parameters' (which is x's or another of the three); statistics and
     sums are float32, dgamma and dbeta are summed in a fixed order."""
     gamma, beta = norm.weight, norm.bias
-    if torch.is_grad_enabled() and (x.requires_grad or (gamma is not None and gamma.requires_grad) or (beta is not None and beta.requires_grad)):
+    if _differentiates(x, gamma, beta):
         return LayerNormRows.apply(x, gamma, beta, norm.normalized_shape, norm.eps)
     x2, ld, p_dtype = _norm_rows(x, gamma, beta, norm.normalized_shape, "layer_norm")
     y = x.new_empty(x.shape)

@@ -80,3 +80,49 @@ def test_backward_steps_by_the_stride_of_the_rows_that_it_gets(op, hook, calls):
     assert not any(a in starts for name, args in calls if name == "snipper_fp8_matmul" for a in args)
     for t in given:
         assert last <= t.untyped_storage().data_ptr() + t.untyped_storage().nbytes()
+
+
+def _differentiable_calls():
+    x, norm, lin = _card(torch.randn(4, 40)), torch.nn.LayerNorm(40), torch.nn.Linear(40, 8)
+    for m in (norm, lin):
+        for n, p in list(m.named_parameters()):
+            setattr(m, n, torch.nn.Parameter(_card(p.detach()), requires_grad=False))
+    return x, norm, lin
+
+
+CALLS = {"layer_norm": lambda x, norm, lin: fused.layer_norm(x, norm), "linear_fp8": lambda x, norm, lin: fp8.linear_fp8(x, lin),
+         "layer_norm_linear_fp8": lambda x, norm, lin: fp8.layer_norm_linear_fp8(x, norm, lin),
+         "quantize_rows": lambda x, norm, lin: fp8.quantize_rows(x), "quantize_both": lambda x, norm, lin: fp8.quantize_both(x),
+         "quantize_tiles": lambda x, norm, lin: fp8.quantize_tiles(x), "layer_norm_fp8": lambda x, norm, lin: fp8.layer_norm_fp8(x, norm)}
+
+
+@pytest.mark.parametrize("grad_mode", [torch.enable_grad, torch.no_grad])
+@pytest.mark.parametrize("op", CALLS)
+def test_forward_mode_derivatives_are_refused_not_dropped(op, grad_mode, calls):
+    """A dual tensor has requires_grad false, and no_grad does not turn forward mode off."""
+    from torch.autograd import forward_ad
+    x, norm, lin = _differentiable_calls()
+    with grad_mode(), forward_ad.dual_level():
+        CALLS[op](x, norm, lin)                                              # (no tangent: as always)
+        made = len(calls)
+        assert made
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            CALLS[op](forward_ad.make_dual(x, torch.ones_like(x)), norm, lin)
+        if op in ("layer_norm", "layer_norm_fp8", "layer_norm_linear_fp8"):
+            norm.weight.requires_grad_(False)
+            dual = torch.nn.LayerNorm(40)
+            del dual.weight
+            dual.weight = forward_ad.make_dual(norm.weight.detach(), torch.ones_like(norm.weight))
+            dual.bias = norm.bias
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                CALLS[op](x, dual, lin)
+
+
+def test_matmul_refuses_a_bias_with_a_tangent(calls):
+    from torch.autograd import forward_ad
+    a = fp8.Fp8Blocks(_card(torch.zeros(4, 128, dtype=torch.float8_e4m3fn)), _card(torch.ones(4, 4, dtype=torch.float32).to(torch.float8_e8m0fnu)), 40)
+    bias = _card(torch.zeros(4))
+    with forward_ad.dual_level():
+        fp8.matmul_fp8(a, a, bias)
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            fp8.matmul_fp8(a, a, forward_ad.make_dual(bias, torch.ones_like(bias)))
