@@ -60,6 +60,7 @@ def test_backward_steps_by_the_stride_of_the_rows_that_it_gets(op, hook, calls):
             setattr(m, n, torch.nn.Parameter(_card(p.detach()), requires_grad=True))
     with torch.autograd.graph.saved_tensors_hooks(pack, keep):
         y = fused.layer_norm(x, norm) if op == "layer_norm" else fp8.layer_norm_linear_fp8(x, norm, lin)
+        forward = len(calls)
         torch.autograd.grad(y, x, torch.ones_like(y))
     c = _layer_norm_backward_call(calls)
     assert (c["rows"], c["cols"]) == (rows, cols) and c["ldx"] >= cols
@@ -77,7 +78,7 @@ def test_backward_steps_by_the_stride_of_the_rows_that_it_gets(op, hook, calls):
             assert t.is_contiguous()
     assert c["rstd"] == c["mean"] + 4 * rows
     starts = {t.data_ptr(): t for t in held if not t.is_contiguous()}
-    assert not any(a in starts for name, args in calls if name == "snipper_fp8_matmul" for a in args)
+    assert not any(a in starts for name, args in calls[forward:] if name == "snipper_fp8_matmul" for a in args)
     for t in given:
         assert last <= t.untyped_storage().data_ptr() + t.untyped_storage().nbytes()
 
@@ -126,3 +127,35 @@ def test_matmul_refuses_a_bias_with_a_tangent(calls):
         fp8.matmul_fp8(a, a, bias)
         with pytest.raises((RuntimeError, NotImplementedError)):
             fp8.matmul_fp8(a, a, forward_ad.make_dual(bias, torch.ones_like(bias)))
+
+
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+def test_nothing_is_written_for_a_backward_pass_that_cannot_come(mode, calls):
+    """Trainable modules under no_grad: x's and W's rows only, and the norm in one launch, straight into blocks."""
+    x, norm, lin = _differentiable_calls()
+    for p in (*norm.parameters(), *lin.parameters()):
+        p.requires_grad_(True)
+    with mode():
+        y = fp8.linear_fp8(x, lin)
+        z = fp8.layer_norm_linear_fp8(x, norm, lin)
+    assert y.shape == z.shape == (4, 8) and not y.requires_grad and not z.requires_grad
+    names = [n for n, _ in calls]
+    assert names == ["snipper_fp8_quantize"] * 2 + ["snipper_fp8_matmul", "snipper_fp8_quantize", "snipper_layernorm_forward", "snipper_fp8_matmul"]
+    for n, args in calls:
+        if n == "snipper_fp8_quantize":
+            data, scale, data_t, scale_t = args[12:16]
+            assert data and scale and data_t is None and scale_t is None
+        elif n == "snipper_layernorm_forward":
+            y, mean, rstd, data, scale = args[9:14]
+            assert data and scale and y is None and mean is None and rstd is None
+
+
+@pytest.mark.parametrize("which", ["x", "norm", "weight", "bias"])
+def test_what_a_backward_pass_reads_is_written_when_it_can_come(which, calls):
+    x, norm, lin = _differentiable_calls()
+    {"x": x, "norm": norm.weight, "weight": lin.weight, "bias": lin.bias}[which].requires_grad_(True)
+    y = fp8.layer_norm_linear_fp8(x, norm, lin)
+    assert y.requires_grad
+    y.backward(torch.ones_like(y))
+    made = [n for n, _ in calls].count("snipper_fp8_matmul")
+    assert made == (1 if which == "bias" else 2)
