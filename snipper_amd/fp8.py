@@ -219,6 +219,8 @@ def _linear_forward(x2, ld, weight, bias, out_dtype, want_wt, want_xt, what, nor
     w2, ldw = _matrix(weight, what)
     M, K = x2.shape
     N = w2.shape[0]
+    if M == 0:
+        return x2.new_empty((0, N), dtype=out_dtype), None
     x_room = _room(M, K)
     xt_room = _room(K, M) if want_xt else 0
     rows = x2.new_empty(x_room + _room(N, K), dtype=torch.uint8)
@@ -300,7 +302,11 @@ def linear_fp8(x: torch.Tensor, lin: torch.nn.Linear, grad_dtype: torch.dtype = 
     fmt = _format(grad_dtype, "linear_fp8")
     weight, bias = lin.weight, lin.bias
     _linear_params(x, weight, bias, "linear_fp8")
-    return LinearFp8.apply(x, weight, bias, fmt)
+    if _differentiates(x, weight, bias):
+        return LinearFp8.apply(x, weight, bias, fmt)
+    x2, ld = _matrix(x, "linear_fp8")
+    y, _ = _linear_forward(x2, ld, weight, bias, x.dtype, False, False, "linear_fp8")
+    return y if x2 is x else y.view(*x.shape[:-1], weight.shape[0])
 
 
 def layer_norm_fp8(x: torch.Tensor, norm: torch.nn.LayerNorm, dtype: torch.dtype = torch.float8_e4m3fn) -> Fp8Blocks:
@@ -314,17 +320,23 @@ def layer_norm_fp8(x: torch.Tensor, norm: torch.nn.LayerNorm, dtype: torch.dtype
     return blocks
 
 
+def _norm_linear_rows(x, gamma, beta, normalized_shape, what):
+    """``_norm_rows`` within the sizes of the products."""
+    x2, ld, p_dtype = _norm_rows(x, gamma, beta, normalized_shape, what)
+    if x2.shape[0] > _MAX_DIM:
+        raise ValueError(f"{what}: up to 2^23 rows")
+    return x2, ld, p_dtype
+
+
 class LayerNormLinearFp8(Function):
     """apply(x, gamma, beta, weight, bias, normalized_shape, eps, grad_fmt): see ``layer_norm_linear_fp8``."""
 
     @staticmethod
     def forward(ctx, x, gamma, beta, weight, bias, normalized_shape, eps, grad_fmt):
         what = "layer_norm_linear_fp8"
-        x2, ld, p_dtype = _norm_rows(x, gamma, beta, normalized_shape, what)
+        x2, ld, p_dtype = _norm_linear_rows(x, gamma, beta, normalized_shape, what)
         M, K = x2.shape
         N = weight.shape[0]
-        if M > _MAX_DIM:
-            raise ValueError(f"{what}: up to 2^23 rows")
         nx, ng, nbt, nw, nb = ctx.needs_input_grad[:5]
         ctx.meta = (M, N, K), (x.dtype, p_dtype, p_dtype, weight.dtype, bias.dtype if bias is not None else None), grad_fmt, x.shape
         if M == 0:
@@ -362,4 +374,9 @@ def layer_norm_linear_fp8(x: torch.Tensor, norm: torch.nn.LayerNorm, lin: torch.
     fmt = _format(grad_dtype, what)
     weight, bias = lin.weight, lin.bias
     _linear_params(x, weight, bias, what)
-    return LayerNormLinearFp8.apply(x, norm.weight, norm.bias, weight, bias, norm.normalized_shape, norm.eps, fmt)
+    gamma, beta = norm.weight, norm.bias
+    if _differentiates(x, gamma, beta, weight, bias):
+        return LayerNormLinearFp8.apply(x, gamma, beta, weight, bias, norm.normalized_shape, norm.eps, fmt)
+    x2, ld, p_dtype = _norm_linear_rows(x, gamma, beta, norm.normalized_shape, what)
+    y, _ = _linear_forward(x2, ld, weight, bias, x.dtype, False, False, what, (None, gamma, beta, p_dtype, norm.eps))
+    return y if x2 is x else y.view(*x.shape[:-1], weight.shape[0])

@@ -410,12 +410,16 @@ def _once_differentiable(backward):
 
 def _has_tangent(*tensors) -> bool:
     """Whether a forward-mode derivative would be lost: a dual tensor's requires_grad is false, and no_grad leaves that mode on."""
-    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _differentiates(*tensors) -> bool:
     """Whether a call on these tensors goes through its autograd function (which refuses forward mode)."""
-    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or _has_tangent(*tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return forward_ad._current_level >= 0 and _has_tangent(*tensors)
 
 
 def _opt(t):
