@@ -1,4 +1,6 @@
-"""Calls of the 8-bit operators and the wide layer norm as programs make them: saved-tensor hooks, inference."""
+"""Calls of the 8-bit operators and the wide layer norm as programs make them: saved-tensor hooks, inference, threads."""
+from concurrent.futures import ThreadPoolExecutor
+
 import pytest
 import torch
 
@@ -69,3 +71,23 @@ def test_inference_gives_the_training_step_s_result(op, dtype, rows, cols):
             assert torch.equal(CALLS[op](x.view(1, rows, 1, cols), norm, lin), y.view(1, rows, 1, -1))
             assert CALLS[op](x[:0], norm, lin).shape == (0, y.shape[1])
         assert not y.requires_grad and torch.equal(y, want)
+
+
+@pytest.mark.parametrize("op", CALLS)
+def test_threads_at_once_each_to_its_end(op):
+    """Two threads on streams of their own; what a thread raises is raised here."""
+    norm, lin = _modules(200, 130)
+    xs = [_x(257, 200, torch.bfloat16, seed) for seed in (1, 2)]
+    g = torch.randn(257, 200, generator=_gen(7)).to(DEV)
+    want = [_step(op, x.requires_grad_(), norm, lin, g) for x in xs]
+    torch.cuda.synchronize()
+
+    def loop(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                got = _step(op, xs[i].detach().requires_grad_(), norm, lin, g)
+                torch.cuda.current_stream().synchronize()
+                assert all(torch.equal(a, b) for a, b in zip(got, want[i]))
+        return 10
+    with ThreadPoolExecutor(2) as pool:
+        assert [f.result() for f in [pool.submit(loop, i) for i in (0, 1)]] == [10, 10]
