@@ -47,7 +47,8 @@ int snipper_fp8_quantize(void *stream, const void *x, int x_dtype, long long ldx
  * A, B and out 16-byte, scale pointers 4-byte aligned.  out [M][N] contiguous, of type out_dtype.
  * A bfloat16 / float16 result comes from the 8-bit matrix instructions, which align the products of a block to their largest and
  * drop what lies 2^13 below it (1.5e-5 of the result's norm, whatever K); a float32 result comes from the bfloat16 ones on exactly
- * converted operands (1e-7; magnitudes under 2^-126 count as zero there), at a quarter of the rate.  M, N, K <= 2^23, M N < 2^40. */
+ * converted operands (1e-7), at a quarter of the rate.  Both hold for scales from end to end of their range: what counts is the size of
+ * the products.  M, N, K <= 2^23, M N < 2^40. */
 size_t snipper_fp8_matmul_workspace_bytes(int M, int N, int K, int out_dtype);
 int snipper_fp8_matmul(void *stream, const uint8_t *A, const uint8_t *a_scale, int a_fmt, const uint8_t *B, const uint8_t *b_scale,
                        int b_fmt, int M, int N, int K, const void *bias, int bias_dtype, int relu, void *out, int out_dtype,

@@ -103,6 +103,28 @@ __device__ __forceinline__ float scale_of(int word, int sel) {
   return __uint_as_float(byte ? byte << 23 : 0x400000u);
 }
 
+// Widened with their scales, elements are exact bfloat16 values and sums of their products float32 ones as long as the scales of both
+// sides lie in 2^-95 .. 2^96 (bytes 32 .. 223: the upper three bits not all alike).  Others (a caller's, or those of magnitudes above
+// 2^104 or below 2^-86) would overflow or vanish in bfloat16 where the product's own scale 2^(ea + eb) need not: there the widened
+// elements stay without their scales, and each block's sum takes both at once (mm_add_scaled).  A workgroup of the tile kernel decides
+// that once, before its loop (1024^3 7.2 -> 7.6 us, 384 x 1024 x 79 000 72 -> 73), the kernel for few rows for each group of steps.
+constexpr unsigned kEachByte = 0x80808080u;
+__device__ __forceinline__ unsigned ordinary_scales(int word) {        // the top bits of the bytes that are ordinary
+  const unsigned t = (unsigned)word ^ ((unsigned)word << 1);
+  return t | (t << 1);
+}
+template <int SEL>
+__device__ __forceinline__ f32x4 mm_add_scaled(f32x4 acc, f32x4 part, int sa, i32x4 sb) {
+  const int ea = (int)(((unsigned)sa >> (8 * SEL)) & 255u);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int eb = (int)(((unsigned)sb[q] >> (8 * SEL)) & 255u);
+    acc[q] += ea == 255 || eb == 255 ? __builtin_nanf("") : __builtin_ldexpf(part[q], ea + eb - 254);
+  }
+  return acc;
+}
+constexpr int kScaleOne = 0x7f7f7f7f;
+
 // the operand of a 16-row tile: 32 elements of a row in a lane
 template <int FMT, bool EXACT>
 struct Operand {
@@ -170,7 +192,8 @@ __global__ __launch_bounds__(64 * WM * WN) void mm_tile_kernel(MmArgs a) {
   static_assert((BM + BN) % (8 * kWaves) == 0 && BM % 8 == 0, "whole DMA instructions of 8 rows");
   constexpr int kDma = (BM + BN) / (8 * kWaves);                // 1 KB instructions of a wave and step
   static_assert((BM + BN) % 64 == 0 && BM % 64 == 0 && (BM + BN) / 64 <= kWaves, "one DMA instruction of 64 scale words a wave");
-  __shared__ __attribute__((aligned(16))) unsigned char smem[2 * kBuf + 2 * kScl];
+  // (one object: with another beside it the compiler waits for the DMA into this one before every read)
+  __shared__ __attribute__((aligned(16))) unsigned char smem[2 * kBuf + 2 * kScl + (EXACT ? 16 : 0)];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave - wm * WN;
@@ -212,19 +235,13 @@ __global__ __launch_bounds__(64 * WM * WN) void mm_tile_kernel(MmArgs a) {
            (unsigned)row * (unsigned)Q, kg * 4);
     }
   };
-  int sa[TM], sb[TN];
-  f32x4 acc[TM][TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
   auto read_frag = [&](const unsigned char *rowp, int key, i32x4 &lo, i32x4 &hi) {
     lo = *(const i32x4 *)(rowp + ((g ^ key) * 16));
     hi = *(const i32x4 *)(rowp + (((g + 4) ^ key) * 16));
   };
   const int key_b = (r & 3) | (r & 4);                          // bit 3 of mm_pair_row(., r) is bit 2 of r
-  auto step = [&](auto sel_c, int kt) {
+  auto step = [&](auto far_c, auto sel_c, int kt, int (&sa)[TM], int (&sb)[TN], f32x4 (&acc)[TM][TN]) {
+    constexpr bool FAR = decltype(far_c)::value;
     constexpr int SEL = decltype(sel_c)::value;
     wait_loads<0>();
     __builtin_amdgcn_s_barrier();
@@ -241,6 +258,26 @@ __global__ __launch_bounds__(64 * WM * WN) void mm_tile_kernel(MmArgs a) {
       for (int j = 0; j < TN; ++j) sb[j] = sc[BM + wn * TN * 16 + mm_pair_row(j, r)];
     }
     const unsigned char *base = smem + (kt & 1) * kBuf;
+    if constexpr (FAR) {
+      const int *sc = (const int *)(smem + 2 * kBuf + ((kt >> 2) & 1) * kScl);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        i32x4 lo, hi;
+        read_frag(base + (BM + wn * TN * 16 + mm_pair_row(j, r)) * 128, key_b, lo, hi);
+        Operand<FB, true> o;
+        o.set(lo, hi, kScaleOne, SEL);
+        const i32x4 eb = *(const i32x4 *)(sc + BM + wn * TN * 16 + mm_pair_row(j, 4 * g));        // rows 4 g .. 4 g + 3 of the pair: neighbours
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          read_frag(base + ((wm * TM + i) * 16 + r) * 128, r & 7, lo, hi);
+          Operand<FA, true> x;
+          x.set(lo, hi, kScaleOne, SEL);
+          acc[i][j] = mm_add_scaled<SEL>(acc[i][j], mm_step<FB, FA, SEL>(o, x, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0), sa[i], eb);
+          __builtin_amdgcn_sched_barrier(0);                    // (one piece at a time: registers)
+        }
+      }
+      return;
+    }
     Operand<FB, EXACT> b[TN];
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
@@ -260,34 +297,77 @@ __global__ __launch_bounds__(64 * WM * WN) void mm_tile_kernel(MmArgs a) {
     }
     if constexpr (EXACT) __builtin_amdgcn_s_setprio(0);
   };
+  auto sums = [&](auto far_c) {
+    int sa[TM], sb[TN];
+    f32x4 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int kt = k_begin; kt < k_end; kt += 4) {
+      step(far_c, std::integral_constant<int, 0>{}, kt, sa, sb, acc);
+      if (kt + 1 < k_end) step(far_c, std::integral_constant<int, 1>{}, kt + 1, sa, sb, acc);
+      if (kt + 2 < k_end) step(far_c, std::integral_constant<int, 2>{}, kt + 2, sa, sb, acc);
+      if (kt + 3 < k_end) step(far_c, std::integral_constant<int, 3>{}, kt + 3, sa, sb, acc);
+    }
+    // a lane's eight consecutive columns of row (l & 15) of each pair of 16 x 16 pieces
+#pragma unroll
+    for (int j = 0; j < TN; j += 2) {
+      const int n = n0 + wn * TN * 16 + j * 16 + 8 * g;
+      float bias[8];
+      if (!a.part) mm_bias(a, n, bias);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const long long m = m0 + (wm * TM + i) * 16 + r;
+        if (m >= a.M) continue;
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) { v[q] = acc[i][j][q]; v[4 + q] = acc[i][j + 1][q]; }
+        if (a.part) store8(a.part + ((long long)split * a.M + m) * a.N + n, a.N - n, v);
+        else mm_store(a, m, n, v, bias);
+      }
+    }
+  };
+  // EXACT: are the scales of the tile's rows, one row a thread, all ordinary ones?  Eight words a time, the first of them on their way
+  // before the first step's rows.  (A choice per group of steps inside the loop cost every product 10 .. 30 %.)
+  const int n_words = ((k_end + 3) >> 2) - (k_begin >> 2);
+  const int *words = nullptr;
+  int w[8];
+  auto look = [&](int at) {                                     // (the last one again behind it: no branches)
+#pragma unroll
+    for (int q = 0; q < 8; ++q) w[q] = words[min(at + q, n_words - 1)];
+  };
+  if constexpr (EXACT) {
+    static_assert(BM + BN <= 64 * kWaves, "a thread for each row");
+    const int row = threadIdx.x % (BM + BN);
+    // (the tile's last row again behind it)
+    words = (const int *)(row < BM ? a.sA + (m0 + min(row, rows_a - 1)) * Q : a.sB + (n0 + min(row - BM, rows_b - 1)) * Q) + (k_begin >> 2);
+    look(0);
+  }
   if (k_begin < k_end) {
     issue(k_begin, k_begin & 1);
     issue_scales(k_begin >> 2);
   }
-  for (int kt = k_begin; kt < k_end; kt += 4) {
-    step(std::integral_constant<int, 0>{}, kt);
-    if (kt + 1 < k_end) step(std::integral_constant<int, 1>{}, kt + 1);
-    if (kt + 2 < k_end) step(std::integral_constant<int, 2>{}, kt + 2);
-    if (kt + 3 < k_end) step(std::integral_constant<int, 3>{}, kt + 3);
-  }
-
-  // a lane's eight consecutive columns of row (l & 15) of each pair of 16 x 16 pieces
+  bool far = false;
+  if constexpr (EXACT) {
+    unsigned usual = kEachByte;
+    for (int at = 0;;) {
 #pragma unroll
-  for (int j = 0; j < TN; j += 2) {
-    const int n = n0 + wn * TN * 16 + j * 16 + 8 * g;
-    float bias[8];
-    if (!a.part) mm_bias(a, n, bias);
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const long long m = m0 + (wm * TM + i) * 16 + r;
-      if (m >= a.M) continue;
-      float v[8];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) { v[q] = acc[i][j][q]; v[4 + q] = acc[i][j + 1][q]; }
-      if (a.part) store8(a.part + ((long long)split * a.M + m) * a.N + n, a.N - n, v);
-      else mm_store(a, m, n, v, bias);
+      for (int q = 0; q < 8; ++q) usual &= ordinary_scales(w[q]);
+      at += 8;
+      if (at >= n_words) break;
+      look(at);
     }
+    static_assert(kWaves == 4, "a word of flags each");
+    int *flags = (int *)(smem + 2 * kBuf + 2 * kScl);
+    if (lane == 0) flags[wave] = 0;
+    if (usual != kEachByte) flags[wave] = 1;
+    __syncthreads();
+    const i32x4 any = *(const i32x4 *)flags;
+    far = (any[0] | any[1] | any[2] | any[3]) != 0;
   }
+  if (EXACT && far) sums(std::integral_constant<bool, EXACT>{});
+  else sums(std::false_type{});
 }
 
 // the splits' sums in a fixed order, then the epilogue; four columns per thread
@@ -456,6 +536,24 @@ __global__ __launch_bounds__(512) void mm_rows_kernel(MmArgs a) {
       b[q][1] = *(const i32x4 *)(bp + at + 16);
       x[q][0] = *(const i32x4 *)(ap + at);
       x[q][1] = *(const i32x4 *)(ap + at + 16);
+    }
+    if constexpr (EXACT) {
+      if (!__all((ordinary_scales(sa) & ordinary_scales(sb) & kEachByte) == kEachByte)) {
+        i32x4 eb;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) eb[q] = __shfl(sb, 4 * g + q, 64);
+        each_step([&](auto step) {
+          constexpr int S = decltype(step)::value;
+          if (kg * 4 + S < a.steps) {
+            Operand<FB, true> o;
+            Operand<FA, true> i;
+            o.set(b[S][0], b[S][1], kScaleOne, S);
+            i.set(x[S][0], x[S][1], kScaleOne, S);
+            acc = mm_add_scaled<S>(acc, mm_step<FB, FA, S>(o, i, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0), sa, eb);
+          }
+        }, std::make_integer_sequence<int, 4>{});
+        continue;
+      }
     }
     each_step([&](auto step) {
       constexpr int S = decltype(step)::value;
