@@ -26,6 +26,8 @@ int launch_status() {
 bool type_ok(int t) { return t == kF32 || t == kBF16 || t == kF16; }
 bool fmt_ok(int f) { return f == 0 || f == 1; }
 bool dim_ok(int n) { return n > 0 && n <= kMaxDim; }
+bool full_sums(int out_dtype) { return out_dtype == kF32 || (out_dtype & SNIPPER_FP8_FULL_SUMS); }
+int element_type(int out_dtype) { return out_dtype & ~SNIPPER_FP8_FULL_SUMS; }
 bool result_ok(int M, int N) { return (long long)M * N < (1ll << 40); }       // (tiles are counted in 32 bits)
 int ceil_div(int a, int b) { return a / b + (a % b != 0); }
 
@@ -166,8 +168,8 @@ int snipper_fp8_quantize(void *stream, const void *x, int x_dtype, long long ldx
 }
 
 size_t snipper_fp8_matmul_workspace_bytes(int M, int N, int K, int out_dtype) {
-  if (!dim_ok(M) || !dim_ok(N) || !dim_ok(K) || !result_ok(M, N) || !type_ok(out_dtype)) return 0;
-  const MmPlan p = mm_plan(M, N, K, out_dtype == kF32);
+  if (!dim_ok(M) || !dim_ok(N) || !dim_ok(K) || !result_ok(M, N) || !type_ok(element_type(out_dtype))) return 0;
+  const MmPlan p = mm_plan(M, N, K, full_sums(out_dtype));
   return p.splits > 1 ? (size_t)p.splits * M * N * sizeof(float) : 0;
 }
 
@@ -175,13 +177,14 @@ int snipper_fp8_matmul(void *stream, const uint8_t *A, const uint8_t *a_scale, i
                        int b_fmt, int M, int N, int K, const void *bias, int bias_dtype, int relu, void *out, int out_dtype,
                        void *workspace, size_t workspace_bytes) {
   if (!A || !a_scale || !B || !b_scale || !out) return SNIPPER_E_NULL;
-  if (!dim_ok(M) || !dim_ok(N) || !dim_ok(K) || !result_ok(M, N) || !fmt_ok(a_fmt) || !fmt_ok(b_fmt) || !type_ok(out_dtype) || !type_ok(bias_dtype)) return SNIPPER_E_SHAPE;
+  if (!dim_ok(M) || !dim_ok(N) || !dim_ok(K) || !result_ok(M, N) || !fmt_ok(a_fmt) || !fmt_ok(b_fmt) || !type_ok(element_type(out_dtype)) || !type_ok(bias_dtype))
+    return SNIPPER_E_SHAPE;
   if (((uintptr_t)A | (uintptr_t)B | (uintptr_t)out) & 15 || ((uintptr_t)a_scale | (uintptr_t)b_scale) & 3) return SNIPPER_E_SHAPE;
-  const bool exact = out_dtype == kF32;
+  const bool exact = full_sums(out_dtype);
   const MmPlan p = mm_plan(M, N, K, exact);
   const size_t need = snipper_fp8_matmul_workspace_bytes(M, N, K, out_dtype);
   if (need && (!workspace || workspace_bytes < need)) return SNIPPER_E_SHAPE;
-  const MmArgs a{A, a_scale, B, b_scale, M, N, ceil_div(K, 128), bias, bias_dtype, relu, out, out_dtype,
+  const MmArgs a{A, a_scale, B, b_scale, M, N, ceil_div(K, 128), bias, bias_dtype, relu, out, element_type(out_dtype),
                  p.splits > 1 ? (float *)workspace : nullptr, p.splits, p.per_split};
   hipStream_t st = (hipStream_t)stream;
   with_fmt(a_fmt, [&](auto fa) {

@@ -4,11 +4,15 @@
 //
 // v_mfma_scale_f32_16x16x128_f8f6f4 multiplies 16 x 128 by 128 x 16 elements with a power-of-two scale for each 32 of a lane's
 // elements: a block of 128 is one instruction whose four scales are the same byte, so scaling costs no instruction at all and any
-// order of the 128 elements within the operands is right as long as both have the same one.  The unit adds the products of an
-// instruction after aligning them to the largest and drops what lies 2^13 or more below it (measured: 1.5e-5 of the result's norm at K
-// = 128 .. 65 536; the sum over blocks is float32): far inside half a step of a bfloat16 (2^-9) or float16 (2^-12) result, but not
-// of a float32 one.  EXACT kernels therefore widen the operands to bfloat16 with their scales -- 4 bits and a power of two fit
-// exactly -- and use v_mfma_f32_16x16x32_bf16 (1e-7), at a quarter of the rate.
+// order of the 128 elements within the operands is right as long as both have the same one.  Its sums: the products of eight neighbours
+// (bytes 8 i .. 8 i + 7 of a lane's operand, here of a row) are aligned to the largest of the eight and cut off at 2^-13 of it, towards
+// zero; the groups and the accumulator are added in float32.  (Found with single products over and under a larger one, every
+// distance, place and sign; the unscaled 16 x 16 x 32 instruction does the same.)  So a group loses less than 7 * 2^-13 = 8.5e-4 of its largest
+// product, an element less than that of sum |a b|, in the worst case: under a quarter of half a step of a bfloat16 (2^-8) of that size, 1.75 half
+// steps of a float16 (2^-11).  On random data 1.5e-5 of the result's norm at K = 128 .. 65 536.  That is the rounding to fewer bits that 16-bit
+// results take for the rate: beside the operands' own, up to 2^-4 of every product, it is small; a caller whose operands are exact can ask
+// for float32 sums (SNIPPER_FP8_FULL_SUMS), and float32 results always have them.  Those EXACT kernels widen the operands to bfloat16
+// with their scales -- 4 bits and a power of two fit exactly -- and use v_mfma_f32_16x16x32_bf16 (1e-7), at a quarter of the rate.
 //
 // Rows of n are the first operand and rows of m the second, so that a lane holds consecutive columns of one row of the result.
 #pragma once

@@ -33,6 +33,7 @@ from .fused import (_ROW_DT, _call, _differentiates, _layer_norm_backward, _laye
 
 _FMT = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}
 _MAX_DIM = 1 << 23
+_FULL_SUMS = 16                        # SNIPPER_FP8_FULL_SUMS
 
 
 class Fp8Blocks:
@@ -161,13 +162,13 @@ def quantize_tiles(w: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn) ->
     return a, b
 
 
-def _product(like, a, a_fmt, b, b_fmt, M, N, K, bias, relu, out_dtype):
-    """act(a b^T + bias) [M, N] on the device of ``like``."""
+def _product(like, a, a_fmt, b, b_fmt, M, N, K, bias, relu, out_dtype, full):
+    """act(a b^T + bias) [M, N] on the device of ``like``; full: _FULL_SUMS or 0."""
     out = like.new_empty((M, N), dtype=out_dtype)
     if M == 0 or N == 0:
         return out
     lib = _lib.load()
-    od = _ROW_DT[out_dtype]
+    od = _ROW_DT[out_dtype] | full
     nbytes = lib.snipper_fp8_matmul_workspace_bytes(M, N, K, od)
     ws = like.new_empty(nbytes // 4, dtype=torch.float32) if nbytes else None
     _call(lib.snipper_fp8_matmul, like.get_device(), a[0], a[1], a_fmt, b[0], b[1], b_fmt, M, N, K, _opt(bias),
@@ -181,11 +182,13 @@ def _check_bias(bias, N, device, what):
 
 
 def matmul_fp8(a: Fp8Blocks, b: Fp8Blocks, bias: Optional[torch.Tensor] = None, relu: bool = False,
-               out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+               out_dtype: torch.dtype = torch.bfloat16, full_sums: bool = False) -> torch.Tensor:
     """act(a @ b.T + bias): a [M, K], b [N, K] in blocks (either type each), bias [N] or None -> [M, N] of ``out_dtype``.
 
-    A bfloat16 / float16 result comes from the 8-bit matrix instructions (relative error of their sums 1.5e-5, far inside the
-    result's own rounding); a float32 result from the bfloat16 ones on exactly widened operands, at a quarter of the rate."""
+    A bfloat16 / float16 result comes from the 8-bit matrix instructions, which cut the products of eight neighbours off at 2^-13 of the
+    largest: before its own rounding an element is off by less than 8.5e-4 of the sum of its products' magnitudes (on random data by
+    1.5e-5 of the result's norm).  With ``full_sums``, and in a float32 result always, the sums are float32 ones (1e-7), from the bfloat16
+    instructions on exactly widened operands at a quarter of the rate."""
     K, ad, bd = a.cols, a.data, b.data
     if K != b.cols:
         raise ValueError(f"matmul_fp8: a {a.shape} and b {b.shape} have rows of different length")
@@ -201,7 +204,8 @@ def matmul_fp8(a: Fp8Blocks, b: Fp8Blocks, bias: Optional[torch.Tensor] = None, 
     if bias is not None:
         _no_graph("matmul_fp8", bias)
         _check_bias(bias, N, ad.device, "matmul_fp8")
-    return _product(ad, _parts(a), _FMT[ad.dtype], _parts(b), _FMT[bd.dtype], M, N, K, bias, int(relu), out_dtype)
+    return _product(ad, _parts(a), _FMT[ad.dtype], _parts(b), _FMT[bd.dtype], M, N, K, bias, int(relu), out_dtype,
+                    _FULL_SUMS if full_sums else 0)
 
 
 def _linear_params(x, weight, bias, what):
@@ -213,7 +217,7 @@ def _linear_params(x, weight, bias, what):
         _check_bias(bias, weight.shape[0], x.device, what)
 
 
-def _linear_forward(x2, ld, weight, bias, out_dtype, want_wt, want_xt, what, norm=None):
+def _linear_forward(x2, ld, weight, bias, out_dtype, want_wt, want_xt, full, what, norm=None):
     """y [M, N] of x2 [M, K] (normalised first with ``norm``), and a buffer of what the backward pass reads: the columns' blocks of the
     input (for dW; in front) and of the weight (for dx)."""
     w2, ldw = _matrix(weight, what)
@@ -238,10 +242,10 @@ def _linear_forward(x2, ld, weight, bias, out_dtype, want_wt, want_xt, what, nor
             _quantize(x2, ld, 0, xr, xt, norm=(stats, gamma, beta, p_dtype))
         else:
             _layer_norm_forward(x2, ld, gamma, beta, p_dtype, eps, None, stats, xr)
-    return _product(x2, xr, 0, wr, 0, M, N, K, bias, 0, out_dtype), keep
+    return _product(x2, xr, 0, wr, 0, M, N, K, bias, 0, out_dtype, full), keep
 
 
-def _linear_backward(g, dims, keep, dtypes, want, grad_fmt):
+def _linear_backward(g, dims, keep, dtypes, want, grad_fmt, full):
     """(dx [M, K] or None, dW or None, db or None) from the gradient [..., N]; dims (M, N, K); dtypes of the three; want = which, the
     first two as in the forward pass."""
     M, N, K = dims
@@ -256,8 +260,8 @@ def _linear_backward(g, dims, keep, dtypes, want, grad_fmt):
     _quantize(g2, ld, grad_fmt, gr, gt, colsum=db, ws=p + g_room + t_room if wb else None, ws_bytes=ws_bytes)
     keep = keep.contiguous() if keep is not None else None          # (saved-tensor hooks may have changed its stride)
     k = keep.data_ptr() if keep is not None else 0
-    dx = _product(g2, gr, grad_fmt, _at(k + (_room(K, M) if ww else 0), K, N), 0, M, K, N, None, 0, dtypes[0]) if wx else None
-    dw = _product(g2, gt, grad_fmt, _at(k, K, M), 0, N, K, M, None, 0, dtypes[1]) if ww else None
+    dx = _product(g2, gr, grad_fmt, _at(k + (_room(K, M) if ww else 0), K, N), 0, M, K, N, None, 0, dtypes[0], full) if wx else None
+    dw = _product(g2, gt, grad_fmt, _at(k, K, M), 0, N, K, M, None, 0, dtypes[1], full) if ww else None
     return dx, dw, db
 
 
@@ -266,46 +270,46 @@ def _zero_grads(g, shapes, dtypes, want):
 
 
 class LinearFp8(Function):
-    """apply(x, weight, bias, grad_fmt): see ``linear_fp8``."""
+    """apply(x, weight, bias, grad_fmt, full): see ``linear_fp8``."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, grad_fmt):
+    def forward(ctx, x, weight, bias, grad_fmt, full):
         x2, ld = _matrix(x, "linear_fp8")
         M, K = x2.shape
         N = weight.shape[0]
-        ctx.meta = (M, N, K), (x.dtype, weight.dtype, bias.dtype if bias is not None else None), grad_fmt, x.shape
+        ctx.meta = (M, N, K), (x.dtype, weight.dtype, bias.dtype if bias is not None else None), grad_fmt, full, x.shape
         if M == 0:
             ctx.save_for_backward()
             return x.new_empty((*x.shape[:-1], N))
-        y, keep = _linear_forward(x2, ld, weight, bias, x.dtype, ctx.needs_input_grad[0], ctx.needs_input_grad[1], "linear_fp8")
+        y, keep = _linear_forward(x2, ld, weight, bias, x.dtype, ctx.needs_input_grad[0], ctx.needs_input_grad[1], full, "linear_fp8")
         ctx.save_for_backward(keep)
         return y if x2 is x else y.view(*x.shape[:-1], N)
 
     @staticmethod
     @_once_differentiable
     def backward(ctx, g):
-        dims, dtypes, grad_fmt, shape = ctx.meta
+        dims, dtypes, grad_fmt, full, shape = ctx.meta
         want = ctx.needs_input_grad[:3]
         if dims[0] == 0:
-            return *_zero_grads(g, (shape, dims[1:], dims[1]), dtypes, want), None
+            return *_zero_grads(g, (shape, dims[1:], dims[1]), dtypes, want), None, None
         keep, = ctx.saved_tensors
-        dx, dw, db = _linear_backward(g, dims, keep, dtypes, want, grad_fmt)
-        return dx.view(shape) if dx is not None and len(shape) != 2 else dx, dw, db, None
+        dx, dw, db = _linear_backward(g, dims, keep, dtypes, want, grad_fmt, full)
+        return dx.view(shape) if dx is not None and len(shape) != 2 else dx, dw, db, None, None
 
 
-def linear_fp8(x: torch.Tensor, lin: torch.nn.Linear, grad_dtype: torch.dtype = torch.float8_e4m3fn) -> torch.Tensor:
+def linear_fp8(x: torch.Tensor, lin: torch.nn.Linear, grad_dtype: torch.dtype = torch.float8_e4m3fn, full_sums: bool = False) -> torch.Tensor:
     """``lin(x)`` with 8-bit products, differentiable: ``dense.big_linear`` in 8 bits.
 
     x [..., K] float32 / bfloat16 / float16 -> [..., N] of x's type; lin's parameters in any of the three, their gradients in theirs.
     y = x W^T + b, dx = g W and dW = g^T x are products of blocks along the axis that each sums over; g is rounded to ``grad_dtype``
-    (e4m3, or e5m2 for more range inside a block); db is the sum of the unrounded g."""
-    fmt = _format(grad_dtype, "linear_fp8")
+    (e4m3, or e5m2 for more range inside a block); db is the sum of the unrounded g.  ``full_sums``: as for ``matmul_fp8``, of all three."""
+    fmt, full = _format(grad_dtype, "linear_fp8"), _FULL_SUMS if full_sums else 0
     weight, bias = lin.weight, lin.bias
     _linear_params(x, weight, bias, "linear_fp8")
     if _differentiates(x, weight, bias):
-        return LinearFp8.apply(x, weight, bias, fmt)
+        return LinearFp8.apply(x, weight, bias, fmt, full)
     x2, ld = _matrix(x, "linear_fp8")
-    y, _ = _linear_forward(x2, ld, weight, bias, x.dtype, False, False, "linear_fp8")
+    y, _ = _linear_forward(x2, ld, weight, bias, x.dtype, False, False, full, "linear_fp8")
     return y if x2 is x else y.view(*x.shape[:-1], weight.shape[0])
 
 
@@ -329,54 +333,54 @@ def _norm_linear_rows(x, gamma, beta, normalized_shape, what):
 
 
 class LayerNormLinearFp8(Function):
-    """apply(x, gamma, beta, weight, bias, normalized_shape, eps, grad_fmt): see ``layer_norm_linear_fp8``."""
+    """apply(x, gamma, beta, weight, bias, normalized_shape, eps, grad_fmt, full): see ``layer_norm_linear_fp8``."""
 
     @staticmethod
-    def forward(ctx, x, gamma, beta, weight, bias, normalized_shape, eps, grad_fmt):
+    def forward(ctx, x, gamma, beta, weight, bias, normalized_shape, eps, grad_fmt, full):
         what = "layer_norm_linear_fp8"
         x2, ld, p_dtype = _norm_linear_rows(x, gamma, beta, normalized_shape, what)
         M, K = x2.shape
         N = weight.shape[0]
         nx, ng, nbt, nw, nb = ctx.needs_input_grad[:5]
-        ctx.meta = (M, N, K), (x.dtype, p_dtype, p_dtype, weight.dtype, bias.dtype if bias is not None else None), grad_fmt, x.shape
+        ctx.meta = (M, N, K), (x.dtype, p_dtype, p_dtype, weight.dtype, bias.dtype if bias is not None else None), grad_fmt, full, x.shape
         if M == 0:
             ctx.save_for_backward()
             return x.new_empty((*x.shape[:-1], N))
         before = nx or ng or nbt                       # something in front of the product wants a gradient
         stats = x.new_empty((2, M), dtype=torch.float32) if before or nw else None
-        y, keep = _linear_forward(x2, ld, weight, bias, x.dtype, before, nw, what, (stats, gamma, beta, p_dtype, eps))
+        y, keep = _linear_forward(x2, ld, weight, bias, x.dtype, before, nw, full, what, (stats, gamma, beta, p_dtype, eps))
         ctx.save_for_backward(keep, *((x2, stats, gamma) if before else (None, None, None)))
         return y if x2 is x else y.view(*x.shape[:-1], N)
 
     @staticmethod
     @_once_differentiable
     def backward(ctx, g):
-        dims, dtypes, grad_fmt, shape = ctx.meta
+        dims, dtypes, grad_fmt, full, shape = ctx.meta
         M, N, K = dims
         want = ctx.needs_input_grad[:5]
         if M == 0:
-            return *_zero_grads(g, (shape, K, K, (N, K), N), dtypes, want), None, None, None
+            return *_zero_grads(g, (shape, K, K, (N, K), N), dtypes, want), None, None, None, None
         nx, ng, nbt, nw, nb = want
         keep, x2, stats, gamma = ctx.saved_tensors
         before = nx or ng or nbt
-        dz, dw, db = _linear_backward(g, dims, keep, (dtypes[0], dtypes[3], dtypes[4]), (before, nw, nb), grad_fmt)
+        dz, dw, db = _linear_backward(g, dims, keep, (dtypes[0], dtypes[3], dtypes[4]), (before, nw, nb), grad_fmt, full)
         dx = dgamma = dbeta = None
         if before:
             dx, dgamma, dbeta = _layer_norm_backward(dz, x2, stats, gamma, dtypes[1], nx, ng or nbt)
-        return (dx.view(shape) if nx and len(shape) != 2 else dx, dgamma if ng else None, dbeta if nbt else None, dw, db, None, None, None)
+        return (dx.view(shape) if nx and len(shape) != 2 else dx, dgamma if ng else None, dbeta if nbt else None, dw, db, None, None, None, None)
 
 
 def layer_norm_linear_fp8(x: torch.Tensor, norm: torch.nn.LayerNorm, lin: torch.nn.Linear,
-                          grad_dtype: torch.dtype = torch.float8_e4m3fn) -> torch.Tensor:
+                          grad_dtype: torch.dtype = torch.float8_e4m3fn, full_sums: bool = False) -> torch.Tensor:
     """``lin(norm(x))``, differentiable, as ``linear_fp8`` after ``fused.layer_norm`` without the norm's result in 16 or 32 bits: it is
     rounded from float32 straight into the blocks that the two products read.  The gradient between the two has x's type."""
     what = "layer_norm_linear_fp8"
-    fmt = _format(grad_dtype, what)
+    fmt, full = _format(grad_dtype, what), _FULL_SUMS if full_sums else 0
     weight, bias = lin.weight, lin.bias
     _linear_params(x, weight, bias, what)
     gamma, beta = norm.weight, norm.bias
     if _differentiates(x, gamma, beta, weight, bias):
-        return LayerNormLinearFp8.apply(x, gamma, beta, weight, bias, norm.normalized_shape, norm.eps, fmt)
+        return LayerNormLinearFp8.apply(x, gamma, beta, weight, bias, norm.normalized_shape, norm.eps, fmt, full)
     x2, ld, p_dtype = _norm_linear_rows(x, gamma, beta, norm.normalized_shape, what)
-    y, _ = _linear_forward(x2, ld, weight, bias, x.dtype, False, False, what, (None, gamma, beta, p_dtype, norm.eps))
+    y, _ = _linear_forward(x2, ld, weight, bias, x.dtype, False, False, full, what, (None, gamma, beta, p_dtype, norm.eps))
     return y if x2 is x else y.view(*x.shape[:-1], weight.shape[0])

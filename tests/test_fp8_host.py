@@ -159,3 +159,33 @@ def test_what_a_backward_pass_reads_is_written_when_it_can_come(which, calls):
     y.backward(torch.ones_like(y))
     made = [n for n, _ in calls].count("snipper_fp8_matmul")
     assert made == (1 if which == "bias" else 2)
+
+
+def test_full_sums_reach_every_product(calls):
+    x, norm, lin = _differentiable_calls()
+    x, lin = x.bfloat16().as_subclass(OnCard).requires_grad_(), lin.requires_grad_()
+    for full in (False, True):
+        del calls[:]
+        for y in (fp8.linear_fp8(x, lin, full_sums=full), fp8.layer_norm_linear_fp8(x, norm, lin, full_sums=full)):
+            y.backward(torch.ones_like(y))
+        types = [args[13] for n, args in calls if n == "snipper_fp8_matmul"]
+        assert types == [1 + 16 * full, 1 + 16 * full, 16 * full] * 2              # y, dx in bfloat16, dW in float32
+    a = fp8.Fp8Blocks(_card(torch.zeros(4, 128, dtype=torch.float8_e4m3fn)), _card(torch.ones(4, 4).to(torch.float8_e8m0fnu)), 40)
+    del calls[:]
+    fp8.matmul_fp8(a, a, out_dtype=torch.float16, full_sums=True)
+    assert calls[0][1][13] == 3 + 16
+
+
+def test_c_matmul_takes_the_flag_of_full_sums():
+    import ctypes
+    lib = _lib.load()
+    p = ctypes.c_void_p(4096)
+    need = lib.snipper_fp8_matmul_workspace_bytes
+    for M, N, K in ((384, 1024, 79000), (1, 4096, 4096), (300, 200, 9000)):
+        assert need(M, N, K, 1 | 16) == need(M, N, K, 3 | 16) == need(M, N, K, 0) == need(M, N, K, 16)
+    assert need(384, 1024, 79000, 2 | 16) == 0 and need(384, 1024, 79000, 32) == 0
+
+    def call(odt, nb=0):
+        return lib.snipper_fp8_matmul(None, p, p, 0, p, p, 0, 384, 1024, 79000, None, 0, 0, p, odt, p if nb else None, nb)
+    assert call(2 | 16) == call(32) == call(64 | 1) == -2
+    assert call(1 | 16) == call(1 | 16, need(384, 1024, 79000, 0) - 1) == -2

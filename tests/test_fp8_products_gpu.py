@@ -1,9 +1,10 @@
-"""8-bit products at the ends of their scales' range, kernel by kernel, against the formula in 64 bits."""
+"""8-bit products where their sums can go wrong, kernel by kernel, against the formula in 64 bits: scales at the ends of their range, a few
+large products beside many small ones, sums that cancel."""
 import pytest
 import torch
 
 from tests import fp8_reference as R
-from snipper_amd import fp8
+from snipper_amd import fp8, fused
 
 pytestmark = pytest.mark.gpu
 E4M3, E5M2 = R.E4M3, R.E5M2
@@ -126,3 +127,88 @@ def test_infinities_and_nan_beside_far_scales(M, N, K, fa):
     assert torch.isfinite(y[rest]).all()
     if fa == E4M3:
         assert torch.equal(y[rest], clean[rest])
+
+
+# ... and those of 16-bit results: tiles of 128, of 256, and the kernel with B in registers
+SHAPES16 = SHAPES + [(4097, 4100, 140), (2111, 2048, 300), (16400, 200, 1000)]
+
+
+def _outliers(rows, K, seed, cancel):
+    """In each group of eight one large element and seven whose products lie just under 2^-13 of the large one's; with ``cancel`` the
+    large ones come in pairs of opposite signs."""
+    g = _gen(seed)
+    d = torch.full((rows, -(-K // 128) * 128), 1.75 * 2.0 ** -7) if cancel else torch.full((rows, -(-K // 128) * 128), 2.0 ** -7)
+    d[:, ::8] = 1
+    if cancel:
+        d[:, 8::16] = -1
+    else:
+        d *= torch.randint(0, 2, d.shape, generator=g) * 2 - 1
+    d[:, K:] = 0
+    s = torch.full((rows, -(-K // 512) * 4), 127, dtype=torch.uint8)
+    s[:, :-(-K // 128)] = torch.randint(124, 130, (rows, 1), generator=g, dtype=torch.uint8)
+    return fp8.Fp8Blocks(d.to(E4M3).to(DEV), s.view(torch.float8_e8m0fnu).to(DEV), K)
+
+
+@pytest.mark.parametrize("out", ["bf16", "f16"])
+@pytest.mark.parametrize("cancel", [True, False])
+@pytest.mark.parametrize("M,N,K", SHAPES16)
+def test_large_products_beside_small_ones(M, N, K, cancel, out):
+    """Each element within what the 8-bit instructions may drop; with full_sums within float32 sums."""
+    a, b = _outliers(M, K, 1, cancel), _outliers(N, K, 2, False)
+    if cancel:
+        b.data.copy_(b.data.float().abs().to(E4M3))
+    y = fp8.matmul_fp8(a, b, out_dtype=DT[out])
+    _check(y, a, b, True)
+    z = fp8.matmul_fp8(a, b, out_dtype=DT[out], full_sums=True)
+    _check(z, a, b, False)
+    if cancel and K % 16 == 0:                  # the small ones are all that is left: 7 / 8 of K products of 1.75 * 2^-14
+        assert not y.any() and (z > 0).all()
+
+
+@pytest.mark.parametrize("out", ["bf16", "f16"])
+@pytest.mark.parametrize("M,N,K", SHAPES16)
+def test_random_products_element_by_element(M, N, K, out):
+    g = _gen(M + K)
+    a, b = R.random_blocks(M, K, E5M2, DEV, g, 3), R.random_blocks(N, K, E4M3, DEV, g, 3)
+    if out == "f16":                            # (in its range)
+        a.scale.view(torch.uint8)[:, :-(-K // 128)] -= 14
+    bias = torch.randn(N, generator=g).to(DEV)
+    for full in (False, True):
+        _check(fp8.matmul_fp8(a, b, bias, relu=full, out_dtype=DT[out], full_sums=full), a, b, not full, bias, relu=full)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_linear_with_full_sums(dtype):
+    """y, dx and dW of outliers whose small neighbours the 8-bit instructions drop; the norm + Linear's are those of its parts."""
+    M, N, K = 160, 48, 256
+    big = _outliers(M, K, 1, True).data.float().to(dtype).requires_grad_()
+    lin, norm = torch.nn.Linear(K, N, device=DEV, dtype=dtype), torch.nn.LayerNorm(K, device=DEV, dtype=dtype)
+    with torch.no_grad():
+        lin.weight.copy_(_outliers(N, K, 2, False).data.float().abs())
+        lin.bias.zero_()
+    gm = _outliers(M, N, 3, True).data.float()[:, :N].to(dtype)
+
+    def step(call):
+        y = call()
+        return (y.detach(), *torch.autograd.grad(y, (big, lin.weight), gm))
+    q = lambda t, tile=1: R.rounded(t.detach().cpu(), E4M3, tile).to(DEV)
+    w8 = q(lin.weight, 128)
+    for got, A, B in zip(step(lambda: fp8.linear_fp8(big, lin, full_sums=True)), (q(big), q(gm), q(gm.t())), (w8, w8.t(), q(big.t()))):
+        e = A @ B.t()
+        assert ((got.double() - e).abs() <= _bound(A, B, e, dtype, False)).all()
+    y = fp8.linear_fp8(big, lin).detach()
+    full = fp8.linear_fp8(big, lin, full_sums=True).detach()
+    assert not y.any() and (full > 0).all()
+    with torch.no_grad():
+        assert torch.equal(full, fp8.linear_fp8(big, lin, full_sums=True))
+    z = fused.layer_norm(big, norm)
+    a = fp8.layer_norm_linear_fp8(big, norm, lin, full_sums=True)
+    blocks, wt = fp8.quantize_rows(torch.nn.functional.layer_norm(big.detach().float(), (K,))), fp8.quantize_tiles(lin.weight.detach())[0]
+    e = R.held(blocks) @ R.held(wt).t()
+    # (the norm's own rounding may move an element to the next value of its type: 2^-3 of it)
+    S = R.held(blocks).abs() @ R.held(wt).abs().t()
+    assert ((a.double() - e).abs() <= torch.finfo(dtype).eps / 2 * e.abs() + 2.0 ** -3 * S).all()
+    dz = torch.autograd.grad(fp8.linear_fp8(z, lin, full_sums=True), z, gm)[0]
+    want = torch.autograd.grad(fused.layer_norm(big, norm), (big, norm.weight, norm.bias), dz)
+    for p, w in zip(torch.autograd.grad(a, (big, norm.weight, norm.bias), gm), want):
+        assert torch.equal(p, w)
