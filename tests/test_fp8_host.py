@@ -169,7 +169,7 @@ def test_full_sums_reach_every_product(calls):
         for y in (fp8.linear_fp8(x, lin, full_sums=full), fp8.layer_norm_linear_fp8(x, norm, lin, full_sums=full)):
             y.backward(torch.ones_like(y))
         types = [args[13] for n, args in calls if n == "snipper_fp8_matmul"]
-        assert types == [1 + 16 * full, 1 + 16 * full, 16 * full] * 2              # y, dx in bfloat16, dW in float32
+        assert types == [1 + 16 * full] * 2 + [1 + 16 * full, 16 * full] * 2       # y, y; dx in bfloat16, dW in float32
     a = fp8.Fp8Blocks(_card(torch.zeros(4, 128, dtype=torch.float8_e4m3fn)), _card(torch.ones(4, 4).to(torch.float8_e8m0fnu)), 40)
     del calls[:]
     fp8.matmul_fp8(a, a, out_dtype=torch.float16, full_sums=True)
