@@ -184,7 +184,7 @@ __device__ __forceinline__ void each_step(F &&f, std::integer_sequence<int, K...
 // consecutive rows, key = r & 7; B: rows of mm_pair_row, key = bits 0, 1 and 3 of r; two buffers, one barrier a step.  The scale words
 // of four K steps come the same way (plain loads of them would make the compiler wait for the DMAs issued after them).
 // 8192^3 in tiles of 256 x 256 by eight waves of 128 x 64: 458 us, 2.4 PFLOP/s, where the instructions alone reach 3.65 .. 4.45 on such
-// data and a large library product 2.98.  A K step takes 64 KB from the L2 into LDS for 33.5 MFLOP a CU, and the LDS reads of its waves
+// data and a large library product 2.98.  A K step takes 64 KB from the L2 into LDS for 16.8 MFLOP a CU, and the LDS reads of its waves
 // and that fill share the LDS; four waves of 128 x 128, which read less, hold half the rows in flight (510 .. 568 us), operands
 // straight from the L2 735, steps of half a block with the 32 x 32 x 64 instruction 558, touching lines a step ahead 491.  EXACT: 79 000
 // x 1024 x 384's weight gradient 72 us = 0.86 PFLOP/s; the bfloat16 instructions' own limit is 43 us, the rest is widening.
