@@ -212,3 +212,79 @@ def test_linear_with_full_sums(dtype):
     want = torch.autograd.grad(fused.layer_norm(big, norm), (big, norm.weight, norm.bias), dz)
     for p, w in zip(torch.autograd.grad(a, (big, norm.weight, norm.bias), gm), want):
         assert torch.equal(p, w)
+
+
+# ---- the kernel with B in registers: K up to 1024 on many rows, N a multiple of 8 ------------------------------------------------------
+def _check_many(y, a, b, bias, relu):
+    """As ``_check`` with what a group drops taken relative to all of its products, for results of many elements."""
+    A, B = R.held(a), R.held(b)
+    e = A @ B.t() + (0 if bias is None else bias.double())
+    S = A.abs() @ B.abs().t() + (0 if bias is None else bias.double().abs())
+    half, K = torch.finfo(y.dtype).eps / 2, A.shape[1]
+    lost = (7 * 2.0 ** -13 + (K / 8 + K / 128 + 64) * 2.0 ** -23) * S
+    bound = half * (e.abs() + lost) + lost + torch.finfo(y.dtype).smallest_normal * half
+    if relu:
+        e = e.clamp(min=0)
+    off = (y.double() - e).abs()
+    assert (off <= bound).all(), (off / bound).max()
+    # and, random as the elements are, near that in the norm: half a step (sqrt 3 below its largest on average), 1e-4 for what is dropped
+    assert off.norm() <= (half / 3 ** 0.5 * 1.1 + 1e-4) * S.norm()
+
+
+@pytest.mark.parametrize("short", [0, 60])
+@pytest.mark.parametrize("steps", range(1, 9))
+def test_many_rows_with_short_k(steps, short):
+    """Each number of K steps (a ring of 4, 3 or 2 slots), each pair of types, more chunks of 64 rows than twice the ring, ragged rows and
+    columns that end inside a wave's 32."""
+    K, M, N = 128 * steps - short, 40007, 1000
+    bias = torch.randn(N, generator=_gen(1)).to(DEV)
+    for i, (fa, fb) in enumerate([(E4M3, E4M3), (E5M2, E4M3), (E4M3, E5M2), (E5M2, E5M2)]):
+        g = torch.Generator(device=DEV).manual_seed(K + i)
+        x = torch.randn(M, K, generator=g, device=DEV) * torch.exp(torch.randn(M, 1, generator=g, device=DEV))
+        w = torch.randn(N, K, generator=g, device=DEV) / K ** 0.5
+        a, b = fp8.quantize_rows(x, fa), fp8.quantize_rows(w, fb)
+        for out, bi, relu in ((torch.bfloat16, bias, i % 2 == 0), (torch.float16, None if i % 2 else bias.to(torch.bfloat16), i % 2 == 1)):
+            y = fp8.matmul_fp8(a, b, bi, relu=relu, out_dtype=out)
+            _check_many(y, a, b, bi, relu)
+            assert torch.equal(y, fp8.matmul_fp8(a, b, bi, relu=relu, out_dtype=out))
+            tail = fp8.Fp8Blocks(a.data[-300:], a.scale[-300:], K)
+            assert torch.equal(y[:, :8], fp8.matmul_fp8(a, fp8.Fp8Blocks(b.data[:8], b.scale[:8], K), None if bi is None else bi[:8], relu=relu, out_dtype=out))
+            _check_many(fp8.matmul_fp8(tail, b, bi, relu=relu, out_dtype=out), tail, b, bi, relu)
+
+
+@pytest.mark.parametrize("M,N,K", [(4100, 4104, 140), (16400, 264, 1000), (20000, 8, 70), (4164, 4104, 400)])
+def test_poisoned_rows_with_b_in_registers(M, N, K):
+    x, w = torch.randn(M, K, generator=_gen(1)).to(DEV), torch.randn(N, K, generator=_gen(2)).to(DEV)
+    clean = fp8.matmul_fp8(fp8.quantize_rows(x, E5M2), fp8.quantize_rows(w))
+    x[1, 7], x[2, K - 1], w[3, 5] = float("nan"), float("inf"), float("nan")
+    x[M - 1, 0] = float("nan")
+    a, b = fp8.quantize_rows(x, E5M2), fp8.quantize_rows(w)
+    a.scale.view(torch.uint8)[3, 0] = 255
+    b.scale.view(torch.uint8)[N - 2, 0] = 255
+    y = fp8.matmul_fp8(a, b)
+    assert all(torch.isnan(y[i]).all() for i in (1, 3, M - 1)) and all(torch.isnan(y[:, j]).all() for j in (3, N - 2))
+    assert not torch.isfinite(y[2]).any()
+    rows, cols = [i for i in range(M) if i not in (1, 2, 3, M - 1)], [j for j in range(N) if j not in (3, N - 2)]
+    assert torch.equal(y[rows][:, cols], clean[rows][:, cols])
+    r = fp8.matmul_fp8(a, b, relu=True)
+    assert torch.isnan(r[1]).all() and torch.isnan(r[:, 3]).all()
+    rest = y[rows][:, cols]
+    assert torch.equal(r[rows][:, cols], rest.clamp(min=0))
+
+
+@pytest.mark.parametrize("kind,grad", [("bf16", E5M2), ("f16", E4M3)])
+def test_linear_of_many_rows(kind, grad):
+    """y and dx from the kernel with B in registers, the gradient in either type, dW over many pieces of a long K axis."""
+    M, N, K = 20011, 136, 264
+    x = (torch.randn(M, K, generator=_gen(1)) * torch.exp(0.5 * torch.randn(M, 1, generator=_gen(2)))).to(DT[kind]).to(DEV).requires_grad_()
+    lin = torch.nn.Linear(K, N, device=DEV)
+    g = (torch.randn(M, N, generator=_gen(3)) * 0.1).to(DT[kind]).to(DEV)
+    y = fp8.linear_fp8(x, lin, grad_dtype=grad)
+    dx, dw, db = torch.autograd.grad(y, (x, lin.weight, lin.bias), g)
+    xq, gq = fp8.quantize_both(x.detach()), fp8.quantize_both(g, grad)
+    w, wt = fp8.quantize_tiles(lin.weight.detach())
+    _check_many(y.detach(), xq[0], w, lin.bias.detach(), False)
+    _check_many(dx, gq[0], wt, None, False)
+    _check(dw, gq[1], xq[1], False)
+    # the longest chain of additions of a sum over rows: 32 rows of a lane and wave, then 157 tiles in 32 slices
+    assert ((db.double() - g.double().sum(0)).abs() <= 128 * 2.0 ** -24 * g.double().abs().sum(0)).all()
