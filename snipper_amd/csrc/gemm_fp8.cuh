@@ -114,8 +114,8 @@ __device__ __forceinline__ float scale_of(int word, int sel) {
 // that once, before its loop (1024^3 7.2 -> 7.6 us, 384 x 1024 x 79 000 72 -> 73), the kernel for few rows for each group of steps.
 constexpr unsigned kEachByte = 0x80808080u;
 __device__ __forceinline__ unsigned ordinary_scales(int word) {        // the top bits of the bytes that are ordinary
-  const unsigned t = (unsigned)word ^ ((unsigned)word << 1);
-  return t | (t << 1);
+  const unsigned w = (unsigned)word, t = w ^ (w << 1);
+  return t | (t << 1) | (((w & ~kEachByte) + 0x01010101u) & w);       // (255, which stands for NaN, is one of them)
 }
 template <int SEL>
 __device__ __forceinline__ f32x4 mm_add_scaled(f32x4 acc, f32x4 part, int sa, i32x4 sb) {

@@ -129,6 +129,26 @@ def test_infinities_and_nan_beside_far_scales(M, N, K, fa):
         assert torch.equal(y[rest], clean[rest])
 
 
+
+@pytest.mark.parametrize("out,full", [("f32", False), ("bf16", False), ("bf16", True)])
+@pytest.mark.parametrize("M,N,K", [(5, 40, 300), (200, 300, 300), (2100, 2090, 300)])
+def test_a_scale_that_stands_for_nan(M, N, K, out, full):
+    """Whatever the elements under it, zeros too; the other rows keep their bits."""
+    g = _gen(K)
+    for kind in ("zeros", "positive", "random"):
+        x, w = torch.randn(M, K, generator=g), torch.randn(N, K, generator=g)
+        if kind != "random":
+            x, w = x.abs(), w.abs()
+        if kind == "zeros":
+            x[3] = 0
+        a, b = fp8.quantize_rows(x.to(DEV)), fp8.quantize_rows(w.to(DEV))
+        clean = fp8.matmul_fp8(a, b, out_dtype=DT[out], **({"full_sums": True} if full else {}))
+        a.scale.view(torch.uint8)[3, 1] = 255
+        y = fp8.matmul_fp8(a, b, out_dtype=DT[out], **({"full_sums": True} if full else {}))
+        assert torch.isnan(y[3]).all()
+        assert torch.equal(torch.cat([y[:3], y[4:]]), torch.cat([clean[:3], clean[4:]]))
+
+
 # ... and those of 16-bit results: tiles of 128, of 256, and the kernel with B in registers
 SHAPES16 = SHAPES + [(4097, 4100, 140), (2111, 2048, 300), (16400, 200, 1000)]
 
