@@ -89,11 +89,14 @@ MmPlan mm_plan(int M, int N, int K, bool exact) {
     return p;
   }
   // K <= 1024: loads and stores bound such products, and the kernel with B in registers overlaps them.  Whole 16-byte pieces of rows
-  // only, and at least as many chunks of 64 rows as there are CUs.  79 000 x 1024 x 384 52 against 100, 16 384 x 1024 x 1024 27 against
-  // 28, 4096 x 4096 x 512 18 against 21; with fewer chunks 1024^3 13 against 6
-  if (!exact && steps <= 8 && N % 8 == 0 && (long long)ceil_div(M, 64) * ceil_div(N, 256) >= kCUs && (long long)N * 128 <= 0x7fffffff) {
+  // only (N = 1001 goes to tiles: 79 000 x 1001 x 384 94, N = 1000 46), at least as many chunks of 64 rows as there are CUs, and no more
+  // than 32 column blocks of 256: chunk lists come in multiples of 8 (one an XCD), and with 33 blocks 8 workgroups are left for a second
+  // round.  Here against the better tile: 79 000 x 1024 x 384 45 / 85, 79 000 x 384 x 1024 44 / 54, 16 384 x 1024 x 1024 24 / 27, 4096 x 4096 x 512
+  // 15 / 21; wide N at K = 1024, 8192 rows: N = 1024 17.7 / 16.9, 2048 24 / 27, 2816 (176 workgroups) 35 / 40, 4096 37 / 50, 4104 (136) 61 / 59, at
+  // K = 384 34 / 40; 8200: 123 / 118 (K = 384: 106 / 86); with fewer chunks 1024^3 13 / 6
+  if (!exact && steps <= 8 && N % 8 == 0 && ceil_div(N, 256) <= kCUs / 8 && (long long)ceil_div(M, 64) * ceil_div(N, 256) >= kCUs) {
     p.kind = 3;
-    p.tiles = std::max(1, kCUs / (8 * ceil_div(N, 256))) * 8;     // chunk lists: one workgroup per CU
+    p.tiles = kCUs / (8 * ceil_div(N, 256)) * 8;     // chunk lists: at most one workgroup per CU
     return p;
   }
   // The largest tile that still gives every CU one: 4096^3 66 (256) against 71 (128); 8192 x 1024 x 4096 38 (128) against 57 (256), 55
@@ -119,7 +122,9 @@ void launch_stationary(const MmArgs &a, int n_series, hipStream_t st) {
   if constexpr (KS < 8) {
     if (a.steps > KS) return launch_stationary<FA, FB, KS + 1>(a, n_series, st);
   }
-  hipLaunchKernelGGL((mm_stationary_kernel<FA, FB, KS>), dim3(n_series * ceil_div(a.N, 256)), dim3(512), 0, st, a, n_series);
+  const dim3 grid(n_series * ceil_div(a.N, 256));
+  if (a.N % 32 == 0) hipLaunchKernelGGL((mm_stationary_kernel<FA, FB, KS, true>), grid, dim3(512), 0, st, a, n_series);
+  else hipLaunchKernelGGL((mm_stationary_kernel<FA, FB, KS, false>), grid, dim3(512), 0, st, a, n_series);
 }
 
 }  // namespace

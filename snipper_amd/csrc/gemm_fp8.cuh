@@ -416,9 +416,10 @@ __device__ __forceinline__ void issue_chunk(const MmArgs &a, unsigned char *slot
 // chunks.  A tile kernel of such shapes spends its time filling and draining: its two or three K steps do not cover the latency of
 // their loads, nor the stores of the tile before.  Here loads run S - 1 chunks ahead across the stores; the counted waits rely on every
 // wave issuing the same number of memory instructions per chunk, so rows and columns past the end go through the buffers' range
-// checks.  The workgroups that share a chunk sit on one XCD: A comes from HBM once.  Results go past the caches: 79 000 x 1024 x 384
-// 54 -> 49 us (tiles of 128 x 128: 100), 193 MB at 3.9 TB/s, nearly all of them stores.
-template <int FA, int FB, int KS>
+// checks.  The workgroups that share a chunk sit on one XCD: A comes from HBM once.  Results go past the caches where the 64 bytes
+// that a wave writes of a row are whole ones in memory (WHOLE: N a multiple of 32): 79 000 x 1024 x 384 54 -> 49 us (tiles of 128 x 128: 90), 193 MB at 3.9 TB/s, nearly
+// all of them stores; elsewhere two waves' pieces meet in the L2 first: N = 1000 101 -> 46 us, 520 48 -> 36 (264 24 -> 25).
+template <int FA, int FB, int KS, bool WHOLE>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void mm_stationary_kernel(MmArgs a, int n_series) {
   constexpr int ROWS = 64, PB = KS * 128, S = KS <= 4 ? 4 : KS <= 6 ? 3 : 2, QW = (KS + 3) / 4, kChunk = ROWS * PB, kScl = ROWS * QW * 4;
   constexpr int kLoads = KS + QW, kStores = 4;
@@ -508,7 +509,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       u32x4 w;
       __builtin_memcpy(&w, h, 16);
       const int n = n0 + 8 * g;
-      __builtin_amdgcn_raw_buffer_store_b128(w, dst, n < a.N ? (unsigned)row * (unsigned)a.N * 2u + (unsigned)n * 2u : 0x80000000u, 0, kPastCaches);
+      const unsigned to = n < a.N ? (unsigned)row * (unsigned)a.N * 2u + (unsigned)n * 2u : 0x80000000u;
+      __builtin_amdgcn_raw_buffer_store_b128(w, dst, to, 0, WHOLE ? kPastCaches : 0);
     }
   }
   wait_loads<0>();                                              // (the empty loads behind the last chunk)

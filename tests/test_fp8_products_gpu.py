@@ -308,3 +308,12 @@ def test_linear_of_many_rows(kind, grad):
     _check(dw, gq[1], xq[1], False)
     # the longest chain of additions of a sum over rows: 32 rows of a lane and wave, then 157 tiles in 32 slices
     assert ((db.double() - g.double().sum(0)).abs() <= 128 * 2.0 ** -24 * g.double().abs().sum(0)).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(700, 8192, 140), (700, 8200, 140), (2111, 2816, 1000), (8003, 520, 300), (8003, 544, 300)])
+def test_wide_results_of_short_k(M, N, K):
+    """On both sides of the number of columns up to which B stays in registers, and rows that are and are not whole pieces of 64 bytes."""
+    g = torch.Generator(device=DEV).manual_seed(N)
+    a, b = (fp8.quantize_rows(torch.randn(r, K, generator=g, device=DEV)) for r in (M, N))
+    bias = torch.randn(N, generator=g, device=DEV)
+    _check_many(fp8.matmul_fp8(a, b, bias), a, b, bias, False)
