@@ -50,7 +50,7 @@ int snipper_fp8_quantize(void *stream, const void *x, int x_dtype, long long ldx
  * less than 7 * 2^-13 (8.5e-4) of the sum of the groups' largest magnitudes, hence of sum |a b|, before it is rounded (half a step of
  * bfloat16 is 2^-8, of float16 2^-11); 1.5e-5 of the result's norm on random data, whatever K.
  * A float32 result comes from the bfloat16 instructions on exactly converted operands (1e-7), at a quarter of the rate; so does a 16-bit
- * one with out_dtype | SNIPPER_FP8_FULL_SUMS.
+ * one of up to 16 rows, or with out_dtype | SNIPPER_FP8_FULL_SUMS.
  * Both hold for scales from end to end of their range: what counts is the size of the products.  M, N, K <= 2^23, M N < 2^40. */
 #define SNIPPER_FP8_FULL_SUMS 16
 size_t snipper_fp8_matmul_workspace_bytes(int M, int N, int K, int out_dtype);

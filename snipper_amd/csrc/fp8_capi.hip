@@ -198,7 +198,7 @@ int snipper_fp8_matmul(void *stream, const uint8_t *A, const uint8_t *a_scale, i
       auto go = [&](auto ex) {
         constexpr bool E = decltype(ex)::value;
         if (p.kind == 0) {
-          hipLaunchKernelGGL((mm_rows_kernel<FA, FB, E>), dim3(ceil_div(N, 16)), dim3(64 * p.waves), 0, st, a);
+          hipLaunchKernelGGL((mm_rows_kernel<FA, FB>), dim3(ceil_div(N, 16)), dim3(64 * p.waves), 0, st, a);
         } else if (p.kind == 4) {
           hipLaunchKernelGGL((mm_tile_kernel<FA, FB, E, 2, 2, 2, 2, false>), dim3(p.tiles * p.splits), dim3(256), 0, st, a);
         } else if (p.kind == 1) {

@@ -517,11 +517,12 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 }
 
 // ---- few rows -----------------------------------------------------------------------------------------------------------
-// At most 16 rows of A: B's bytes count, and they are read once, straight into registers.  A workgroup of W waves makes 16 columns; the
+// At most 16 rows of A: B's bytes count, and they are read once, straight into registers; the sums are full ones for every type of result,
+// since widening costs nothing beside the loads (1 x 8192 x 8192 15.7 us with the 8-bit instructions, 15.0 so).  A workgroup of W waves makes 16 columns; the
 // waves take every W-th group of four K steps (a word of scales; all of a group's loads are on the way before its first product) and
 // add their sums through LDS in a fixed order.  Bound by latency and HBM: 1 x 4096 x 4096 6.6 us (17 MB, 2.5 TB/s), 1 x 8192 x 8192 15 us
 // (67 MB, 4.5 TB/s).
-template <int FA, int FB, bool EXACT>
+template <int FA, int FB>
 __global__ __launch_bounds__(512) void mm_rows_kernel(MmArgs a) {
   __shared__ f32x4 red[8][64];
   const int lane = threadIdx.x & 63, W = blockDim.x >> 6;
@@ -543,29 +544,27 @@ __global__ __launch_bounds__(512) void mm_rows_kernel(MmArgs a) {
       x[q][0] = *(const i32x4 *)(ap + at);
       x[q][1] = *(const i32x4 *)(ap + at + 16);
     }
-    if constexpr (EXACT) {
-      if (!__all((ordinary_scales(sa) & ordinary_scales(sb) & kEachByte) == kEachByte)) {
-        i32x4 eb;
+    if (!__all((ordinary_scales(sa) & ordinary_scales(sb) & kEachByte) == kEachByte)) {
+      i32x4 eb;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) eb[q] = __shfl(sb, 4 * g + q, 64);
-        each_step([&](auto step) {
-          constexpr int S = decltype(step)::value;
-          if (kg * 4 + S < a.steps) {
-            Operand<FB, true> o;
-            Operand<FA, true> i;
-            o.set(b[S][0], b[S][1], kScaleOne, S);
-            i.set(x[S][0], x[S][1], kScaleOne, S);
-            acc = mm_add_scaled<S>(acc, mm_step<FB, FA, S>(o, i, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0), sa, eb);
-          }
-        }, std::make_integer_sequence<int, 4>{});
-        continue;
-      }
+      for (int q = 0; q < 4; ++q) eb[q] = __shfl(sb, 4 * g + q, 64);
+      each_step([&](auto step) {
+        constexpr int S = decltype(step)::value;
+        if (kg * 4 + S < a.steps) {
+          Operand<FB, true> o;
+          Operand<FA, true> i;
+          o.set(b[S][0], b[S][1], kScaleOne, S);
+          i.set(x[S][0], x[S][1], kScaleOne, S);
+          acc = mm_add_scaled<S>(acc, mm_step<FB, FA, S>(o, i, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0), sa, eb);
+        }
+      }, std::make_integer_sequence<int, 4>{});
+      continue;
     }
     each_step([&](auto step) {
       constexpr int S = decltype(step)::value;
       if (kg * 4 + S < a.steps) {
-        Operand<FB, EXACT> o;
-        Operand<FA, EXACT> i;
+        Operand<FB, true> o;
+        Operand<FA, true> i;
         o.set(b[S][0], b[S][1], sb, S);
         i.set(x[S][0], x[S][1], sa, S);
         acc = mm_step<FB, FA, S>(o, i, acc, sb, sa);

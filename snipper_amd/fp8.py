@@ -187,8 +187,8 @@ def matmul_fp8(a: Fp8Blocks, b: Fp8Blocks, bias: Optional[torch.Tensor] = None, 
 
     A bfloat16 / float16 result comes from the 8-bit matrix instructions, which cut the products of eight neighbours off at 2^-13 of the
     largest: before its own rounding an element is off by less than 8.5e-4 of the sum of its products' magnitudes (on random data by
-    1.5e-5 of the result's norm).  With ``full_sums``, and in a float32 result always, the sums are float32 ones (1e-7), from the bfloat16
-    instructions on exactly widened operands at a quarter of the rate."""
+    1.5e-5 of the result's norm).  With ``full_sums``, and always in a float32 result or one of up to 16 rows, the sums are float32 ones (1e-7), from
+    the bfloat16 instructions on exactly widened operands at a quarter of the rate."""
     K, ad, bd = a.cols, a.data, b.data
     if K != b.cols:
         raise ValueError(f"matmul_fp8: a {a.shape} and b {b.shape} have rows of different length")

@@ -59,7 +59,7 @@ def test_saved_tensors_that_come_back_in_another_layout(op, rows, cols, skip):
 
 @pytest.mark.parametrize("op", CALLS)
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 130), (40, 384), (129, 1000), (70, 2100)])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 130), (40, 384), (129, 1000), (70, 2100), (33, 100), (9, 1500), (5, 5000), (3, 9000)])
 def test_inference_gives_the_training_step_s_result(op, dtype, rows, cols):
     norm, lin = _modules(cols, 60)
     x = _x(rows, cols, dtype)

@@ -81,7 +81,7 @@ def test_scales_from_end_to_end_of_their_range(M, N, K, out, fa, fb):
     bias = torch.randn(N, generator=_gen(1)).to(DEV)
     for bi in (None, bias):
         y = fp8.matmul_fp8(a, b, bi, out_dtype=DT[out])
-        _check(y, a, b, out != "f32", bi)
+        _check(y, a, b, out != "f32" and M > 16, bi)          # (up to 16 rows: float32 sums for every type)
         assert torch.equal(y, fp8.matmul_fp8(a, b, bi, out_dtype=DT[out]))
 
 
@@ -178,7 +178,7 @@ def test_large_products_beside_small_ones(M, N, K, cancel, out):
     if cancel:
         b.data.copy_(b.data.float().abs().to(E4M3))
     y = fp8.matmul_fp8(a, b, out_dtype=DT[out])
-    _check(y, a, b, True)
+    _check(y, a, b, M > 16)
     z = fp8.matmul_fp8(a, b, out_dtype=DT[out], full_sums=True)
     _check(z, a, b, False)
     if cancel and K % 16 == 0:                  # the small ones are all that is left: 7 / 8 of K products of 1.75 * 2^-14
@@ -194,7 +194,7 @@ def test_random_products_element_by_element(M, N, K, out):
         a.scale.view(torch.uint8)[:, :-(-K // 128)] -= 14
     bias = torch.randn(N, generator=g).to(DEV)
     for full in (False, True):
-        _check(fp8.matmul_fp8(a, b, bias, relu=full, out_dtype=DT[out], full_sums=full), a, b, not full, bias, relu=full)
+        _check(fp8.matmul_fp8(a, b, bias, relu=full, out_dtype=DT[out], full_sums=full), a, b, M > 16 and not full, bias, relu=full)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
