@@ -26,7 +26,8 @@ __host__ __device__ __forceinline__ long long pitch_of(int cols) { return (long 
 __host__ __device__ __forceinline__ long long scales_of(int cols) { return (long long)((cols + 511) / 512) * 4; }
 
 // ---- rows only.  A wave takes 512 consecutive elements of a row, 8 per lane: four blocks, so that it writes a whole 32-bit word of
-// scales; 16 lanes share a block.
+// scales; 16 lanes share a block.  79 000 x 1024 bf16 43.5 us (5.6 TB/s), 79 000 x 384 float32 28.6 (5.3 TB/s), 16 384 x 8192 bf16 77.6 (5.2
+// TB/s).  A row's last piece leaves lanes idle: 131 072 x 100 bf16 42 us (0.9 TB/s).
 template <typename T, int FMT>
 __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs a) {
   const int lane = threadIdx.x & 63;
