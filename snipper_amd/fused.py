@@ -428,6 +428,8 @@ def _opt(t):
 
 def _row_stride(x2: torch.Tensor):
     """x2 [rows, C], copied unless it has unit stride inside a row and rows that do not overlap, and its row stride."""
+    if x2.is_neg():                                    # (a gradient through conj and imag: its memory holds the opposite signs)
+        x2 = x2.resolve_neg()
     R, C = x2.shape
     ld, inner = x2.stride()
     if R <= 1 and inner == 1:
@@ -515,8 +517,8 @@ class LayerNormRows(Function):
         x2, stats, gamma = ctx.saved_tensors
         p_dtype, shape = ctx.meta
         wx, wg, wb = ctx.needs_input_grad[:3]
-        if g.dtype is not x2.dtype or not g.is_contiguous():
-            g = g.to(x2.dtype).contiguous()
+        if g.dtype is not x2.dtype or not g.is_contiguous() or g.is_neg():
+            g = g.to(x2.dtype).contiguous().resolve_neg()
         dx, dgamma, dbeta = _layer_norm_backward(g, x2, stats, gamma, p_dtype, wx, wg or wb)
         return dx.view(shape) if wx and len(shape) != 2 else dx, dgamma if wg else None, dbeta if wb else None, None, None
 

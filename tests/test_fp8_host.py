@@ -1,4 +1,6 @@
 """What the 8-bit operators' and the wide layer norm's wrappers hand to the native entries, on the CPU: the calls are recorded, not made."""
+import ctypes
+
 import pytest
 import torch
 
@@ -177,7 +179,6 @@ def test_full_sums_reach_every_product(calls):
 
 
 def test_c_matmul_takes_the_flag_of_full_sums():
-    import ctypes
     lib = _lib.load()
     p = ctypes.c_void_p(4096)
     need = lib.snipper_fp8_matmul_workspace_bytes
@@ -189,3 +190,47 @@ def test_c_matmul_takes_the_flag_of_full_sums():
         return lib.snipper_fp8_matmul(None, p, p, 0, p, p, 0, 384, 1024, 79000, None, 0, 0, p, odt, p if nb else None, nb)
     assert call(2 | 16) == call(32) == call(64 | 1) == -2
     assert call(1 | 16) == call(1 | 16, need(384, 1024, 79000, 0) - 1) == -2
+
+
+def _first_values(monkeypatch):
+    """The first float32 of the matrix that each native call reads, as the call finds it in memory."""
+    seen = []
+
+    def record(fn, index, *args):
+        at = {"snipper_fp8_quantize": 0, "snipper_layernorm_forward": 0, "snipper_layernorm_backward": 0}.get(fn.__name__)
+        if at is not None and args[at]:
+            seen.append(ctypes.c_float.from_address(args[at]).value)
+    _lib.load()
+    for module in (fused, fp8):
+        monkeypatch.setattr(module, "_call", record)
+    return seen
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 1), (5, 7)])
+@pytest.mark.parametrize("op", CALLS)
+def test_a_lazily_negated_tensor_is_read_with_its_own_signs(op, rows, cols, monkeypatch):
+    """conj().imag is a view whose memory holds the opposite signs, with or without another stride."""
+    seen = _first_values(monkeypatch)
+    norm, lin = torch.nn.LayerNorm(cols), torch.nn.Linear(cols, 8)
+    for m in (norm, lin):
+        for n, p in list(m.named_parameters()):
+            setattr(m, n, torch.nn.Parameter(_card(p.detach().abs() + 1), requires_grad=False))
+    for x in (torch._neg_view(torch.rand(rows, cols) + 1), (torch.rand(rows, cols, dtype=torch.complex64) + 1 + 1j).conj().imag):
+        del seen[:]
+        assert x.is_neg() and (x < 0).all()
+        CALLS[op](_card(x), norm, lin)
+        assert min(seen) == x[0, 0].item()                                  # (the weight's are above 1)
+
+
+@pytest.mark.parametrize("rows", [1, 3])
+@pytest.mark.parametrize("op", ["layer_norm", "linear_fp8"])
+def test_a_lazily_negated_gradient_is_read_with_its_own_signs(op, rows, monkeypatch):
+    seen = _first_values(monkeypatch)
+    x, norm, lin = _card(torch.randn(rows, 1)).requires_grad_(), torch.nn.LayerNorm(1), torch.nn.Linear(1, 1)
+    for m in (norm, lin):
+        for n, p in list(m.named_parameters()):
+            setattr(m, n, torch.nn.Parameter(_card(p.detach()), requires_grad=False))
+    y = CALLS[op](x, norm, lin)
+    del seen[:]
+    torch.autograd.grad(y, x, _card(torch._neg_view(torch.rand(rows, 1) + 1)))
+    assert seen and seen[0] < 0
