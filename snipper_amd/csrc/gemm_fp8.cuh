@@ -12,7 +12,8 @@
 // steps of a float16 (2^-11).  On random data 1.5e-5 of the result's norm at K = 128 .. 65 536.  That is the rounding to fewer bits that 16-bit
 // results take for the rate: beside the operands' own, up to 2^-4 of every product, it is small; a caller whose operands are exact can ask
 // for float32 sums (SNIPPER_FP8_FULL_SUMS), and float32 results always have them.  Those EXACT kernels widen the operands to bfloat16
-// with their scales -- 4 bits and a power of two fit exactly -- and use v_mfma_f32_16x16x32_bf16 (1e-7), at a quarter of the rate.
+// with their scales -- 4 bits and a power of two fit exactly -- and use v_mfma_f32_16x16x32_bf16 (1e-7), at a quarter of the rate (4096^3
+// 66 us with the 8-bit instructions, 119 so; 384 x 1024 x 79 000 62 and 73; 480 x 1024 x 384 4.7 and 5.2).
 //
 // Rows of n are the first operand and rows of m the second, so that a lane holds consecutive columns of one row of the result.
 #pragma once
@@ -111,7 +112,8 @@ __device__ __forceinline__ float scale_of(int word, int sel) {
 // sides lie in 2^-95 .. 2^96 (bytes 32 .. 223: the upper three bits not all alike).  Others (a caller's, or those of magnitudes above
 // 2^104 or below 2^-86) would overflow or vanish in bfloat16 where the product's own scale 2^(ea + eb) need not: there the widened
 // elements stay without their scales, and each block's sum takes both at once (mm_add_scaled).  A workgroup of the tile kernel decides
-// that once, before its loop (1024^3 7.2 -> 7.6 us, 384 x 1024 x 79 000 72 -> 73), the kernel for few rows for each group of steps.
+// that once, before its loop (1024^3 7.2 -> 7.6 us, 384 x 1024 x 79 000 72 -> 73), the kernel for few
+// rows for each group of steps; a tile of such scales takes 1.8 times as long.
 constexpr unsigned kEachByte = 0x80808080u;
 __device__ __forceinline__ unsigned ordinary_scales(int word) {        // the top bits of the bytes that are ordinary
   const unsigned w = (unsigned)word, t = w ^ (w << 1);
